@@ -299,6 +299,57 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
                                      void *y8, int32_t out_mode, int32_t act, int64_t M, int64_t N,
                                      int64_t K, int32_t terms, void *stream);
 
+/* 8-bit operands with a scale per block, and products grouped by expert. Device pointers on the
+ * current device; all return after enqueueing on `stream`, allocate nothing on it and can be
+ * captured. None has a counterpart in the reference (it has one FP32 product per layer).
+ *
+ * tsfm_kernel_quantize_e4m3: x [rows, cols] (F32, F16 or BF16, row stride ldx elements) to E4M3
+ *   codes q [rows, cols] (bytes, row stride ldq) and one FP32 scale per block of block_rows x 128
+ *   elements (block_rows 1: activations; 128: weights; blocks at the edges are smaller), scale
+ *   [ceil(rows / block_rows), ceil(cols / 128)] with row stride ld_scale. x[r, c] ~ q[r, c] * scale:
+ *   the scale is the smallest power of two with max|x| / scale <= 448 (at least 2^-126), q =
+ *   x / scale rounded to nearest even. A block that holds an infinity or a NaN gets scale and codes
+ *   NaN. rows may be 0.
+ *
+ * tsfm_kernel_linear_e4m3: y[M, N] (+)= act(x W^T + bias) of E4M3 operands x [M, K] and W [N, K]
+ *   (row strides ldx, ldw in bytes, both and the bases 16-byte aligned; K itself may be odd) with
+ *   scales x_scale [M, ceil(K / 128)] (row stride ld_xs; one per 128 elements of a row) and w_scale
+ *   [ceil(N / 128), ceil(K / 128)] (row stride ld_ws; one per 128 x 128 block), any FP32 values:
+ *   y[m, n] = sum_b x_scale[m, b] w_scale[n / 128, b] sum_{k in block b} x[m, k] W[n, k], sums in
+ *   FP32. y_dtype F32, F16 or BF16 (row stride ldy elements, any alignment of the element type);
+ *   accumulate (F32 only) adds to y, and the activation then applies to the sum. act: 0 none, 1 relu,
+ *   3 gated pairs as in tsfm_kernel_linear (N % 256 == 0, 16-bit y of N / 2 columns, no bias).
+ *   bias [N] or null. M may be 0. y overlaps no input.
+ *
+ * tsfm_kernel_linear_grouped: y[r] (+)= act(x[r] W[e]^T + bias[e]) for the rows offsets[e] <= r <
+ *   offsets[e + 1] of group e, 0 <= e < groups (at most 1024). x [M, K], W [groups, N, K] (row stride
+ *   ldw, group stride w_group elements) both BF16 or both F16, bases and strides 16-byte aligned;
+ *   bias [groups, N] or null; y, accumulate and act as above. offsets: groups + 1 int32 in device
+ *   memory, nondecreasing, any group may be empty. Rows of y outside [offsets[0], offsets[groups])
+ *   are left as they were. Offsets outside [0, M] are clamped to it, and one below an earlier one is
+ *   read as that one (its group is empty): no offsets reach outside x and y.
+ *
+ * tsfm_kernel_linear_grouped_e4m3: the same of E4M3 operands, with x_scale [M, ceil(K / 128)] and
+ *   w_scale [groups, ceil(N / 128), ceil(K / 128)] (row stride ld_ws, group stride ws_group). */
+int32_t tsfm_kernel_quantize_e4m3(const void *x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t ldx,
+                                  int32_t block_rows, void *q, int64_t ldq, float *scale,
+                                  int64_t ld_scale, void *stream);
+int32_t tsfm_kernel_linear_e4m3(const void *x, const float *x_scale, int64_t ld_xs, const void *w,
+                                const float *w_scale, int64_t ld_ws, const float *bias, void *y,
+                                int32_t y_dtype, int32_t accumulate, int32_t act, int64_t M, int64_t N,
+                                int64_t K, int64_t ldx, int64_t ldw, int64_t ldy, void *stream);
+int32_t tsfm_kernel_linear_grouped(const void *x, int32_t x_dtype, const void *w, int32_t w_dtype,
+                                   const float *bias, void *y, int32_t y_dtype, int32_t accumulate,
+                                   int32_t act, const int32_t *offsets, int64_t groups, int64_t M,
+                                   int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t w_group,
+                                   int64_t ldy, void *stream);
+int32_t tsfm_kernel_linear_grouped_e4m3(const void *x, const float *x_scale, int64_t ld_xs, const void *w,
+                                        const float *w_scale, int64_t ld_ws, int64_t ws_group,
+                                        const float *bias, void *y, int32_t y_dtype, int32_t accumulate,
+                                        int32_t act, const int32_t *offsets, int64_t groups, int64_t M,
+                                        int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t w_group,
+                                        int64_t ldy, void *stream);
+
 /* tsfm_test_bounded_wait: the failure-detection check of the device waits. Every wait of the
  * warp-specialised kernels (TMA and tensor-core barriers) gives up after 2 s, records its site in
  * the device error word and lets the kernel return, and the host reports

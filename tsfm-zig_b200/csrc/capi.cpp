@@ -67,11 +67,17 @@ int *kernel_err_word() {
     if (dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lk(mu);
     if (!words[dev]) {
+        // The first call on a device may come from a thread that captures a graph: the allocation runs
+        // in the relaxed capture mode, and the clearing on a stream of its own.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
         void *p = nullptr;
-        if (cudaMalloc(&p, 16) == cudaSuccess) {
-            cudaMemset(p, 0, 16);
+        cudaStream_t s = nullptr;
+        if (cudaMalloc(&p, 16) == cudaSuccess && cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess &&
+            cudaMemsetAsync(p, 0, 16, s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess)
             words[dev] = static_cast<int *>(p);
-        }
+        if (s) cudaStreamDestroy(s);
+        cudaThreadExchangeStreamCaptureMode(&mode);
     }
     return words[dev];
 }
@@ -693,6 +699,150 @@ int32_t tsfm_kernel_linear_f16c(const void *x16, const void *x8, const void *w16
         c.y8 = y8;
         c.ldy8 = 2 * N;
         return launch_linear(c, static_cast<cudaStream_t>(stream));
+    });
+}
+
+// Argument checks shared by the block-scaled and the grouped products, then the launch.
+static Status linear_blocks_entry(LinearBlocksCall &c, int64_t groups, int32_t y_dtype, int32_t accumulate, int32_t act,
+                                  cudaStream_t stream) {
+    const bool f8 = c.dtype == E_U8;
+    if (c.M < 0 || c.N <= 0 || c.K <= 0 || groups <= 0) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: bad shape");
+    if (c.M > INT32_MAX - 512 || c.N > INT32_MAX - 512 || c.K > INT32_MAX - 512)
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: dimension exceeds the TMA coordinate range");
+    if (y_dtype != TSFM_DTYPE_F32 && y_dtype != TSFM_DTYPE_F16 && y_dtype != TSFM_DTYPE_BF16)
+        return Status::fail(TSFM_ERR_UNSUPPORTED_DTYPE, "linear: y must be F32, F16 or BF16");
+    if ((act != 0 && act != 1 && act != ACT_GLU) || (accumulate != 0 && accumulate != 1))
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: bad accumulate / act");
+    if (accumulate && y_dtype != TSFM_DTYPE_F32)
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: only an F32 y accumulates");
+    if (act == ACT_GLU && (c.N % 256 || y_dtype == TSFM_DTYPE_F32 || c.bias))
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: gated pairs need N % 256 == 0, a 16-bit y and no bias");
+    const int64_t ycols = act == ACT_GLU ? c.N / 2 : c.N, kb = (c.K + 127) / 128;
+    if (c.ldx < c.K || c.ldw < c.K || c.ldy < ycols || (groups > 1 && c.w_group < (c.N - 1) * c.ldw + c.K))
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: a stride is shorter than its rows");
+    if (f8 && (!c.xs || !c.ws || c.ld_xs < kb || c.ld_ws < kb ||
+               (groups > 1 && c.ws_group < ((c.N + 127) / 128 - 1) * c.ld_ws + kb)))
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: bad scales");
+    const int esz = f8 ? 1 : 2, ysz = y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
+    const auto off = [](const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
+    if (off(c.x, 16) || off(c.w, 16) || (c.ldx * esz) % 16 || (c.ldw * esz) % 16 || (groups > 1 && (c.w_group * esz) % 16))
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: operand base and strides must be 16-byte aligned");
+    if (off(c.y, ysz) || off(c.bias, 4) || off(c.xs, 4) || off(c.ws, 4) || off(c.offsets, 4))
+        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: misaligned pointer");
+    c.groups = groups;
+    c.y_dtype = y_dtype;
+    c.accumulate = accumulate != 0;
+    c.act = act;
+    if (c.M == 0) return Status::ok();
+    c.err = kernel_err_word();
+    return launch_linear_blocks(c, stream);
+}
+
+int32_t tsfm_kernel_quantize_e4m3(const void *x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t ldx,
+                                  int32_t block_rows, void *q, int64_t ldq, float *scale, int64_t ld_scale, void *stream) {
+    return guarded([&]() -> Status {
+        if (!x || !q || !scale) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        if (x_dtype != TSFM_DTYPE_F32 && x_dtype != TSFM_DTYPE_F16 && x_dtype != TSFM_DTYPE_BF16)
+            return Status::fail(TSFM_ERR_UNSUPPORTED_DTYPE, "quantize: x must be F32, F16 or BF16");
+        if (rows < 0 || cols <= 0 || rows > INT32_MAX || cols > INT32_MAX || ldx < cols || ldq < cols ||
+            ld_scale < (cols + 127) / 128 || (block_rows != 1 && block_rows != 128))
+            return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "quantize: bad shape, stride or block_rows");
+        if (reinterpret_cast<uintptr_t>(x) % (x_dtype == TSFM_DTYPE_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scale) % 4)
+            return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "quantize: misaligned pointer");
+        QuantizeCall c;
+        c.x = x;
+        c.x_dtype = x_dtype == TSFM_DTYPE_F32 ? E_F32X : x_dtype == TSFM_DTYPE_F16 ? E_F16 : E_BF16;
+        c.rows = rows;
+        c.cols = cols;
+        c.ldx = ldx;
+        c.block_rows = block_rows;
+        c.q = static_cast<uint8_t *>(q);
+        c.ldq = ldq;
+        c.scale = scale;
+        c.ld_scale = ld_scale;
+        return launch_quantize_e4m3(c, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t tsfm_kernel_linear_e4m3(const void *x, const float *x_scale, int64_t ld_xs, const void *w, const float *w_scale,
+                                int64_t ld_ws, const float *bias, void *y, int32_t y_dtype, int32_t accumulate,
+                                int32_t act, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldy,
+                                void *stream) {
+    return guarded([&]() -> Status {
+        if (!x || !w || !y) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        LinearBlocksCall c;
+        c.x = x;
+        c.w = w;
+        c.dtype = E_U8;
+        c.M = M;
+        c.N = N;
+        c.K = K;
+        c.ldx = ldx;
+        c.ldw = ldw;
+        c.xs = x_scale;
+        c.ld_xs = ld_xs;
+        c.ws = w_scale;
+        c.ld_ws = ld_ws;
+        c.bias = bias;
+        c.y = y;
+        c.ldy = ldy;
+        return linear_blocks_entry(c, 1, y_dtype, accumulate, act, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t tsfm_kernel_linear_grouped(const void *x, int32_t x_dtype, const void *w, int32_t w_dtype, const float *bias,
+                                   void *y, int32_t y_dtype, int32_t accumulate, int32_t act, const int32_t *offsets,
+                                   int64_t groups, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw,
+                                   int64_t w_group, int64_t ldy, void *stream) {
+    return guarded([&]() -> Status {
+        if (!x || !w || !y || !offsets) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        if (x_dtype != w_dtype || (x_dtype != TSFM_DTYPE_BF16 && x_dtype != TSFM_DTYPE_F16))
+            return Status::fail(TSFM_ERR_UNSUPPORTED_DTYPE, "linear: x and w must both be BF16 or F16");
+        LinearBlocksCall c;
+        c.x = x;
+        c.w = w;
+        c.dtype = x_dtype == TSFM_DTYPE_F16 ? E_F16 : E_BF16;
+        c.M = M;
+        c.N = N;
+        c.K = K;
+        c.ldx = ldx;
+        c.ldw = ldw;
+        c.offsets = offsets;
+        c.w_group = w_group;
+        c.bias = bias;
+        c.y = y;
+        c.ldy = ldy;
+        return linear_blocks_entry(c, groups, y_dtype, accumulate, act, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t tsfm_kernel_linear_grouped_e4m3(const void *x, const float *x_scale, int64_t ld_xs, const void *w,
+                                        const float *w_scale, int64_t ld_ws, int64_t ws_group, const float *bias, void *y,
+                                        int32_t y_dtype, int32_t accumulate, int32_t act, const int32_t *offsets,
+                                        int64_t groups, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw,
+                                        int64_t w_group, int64_t ldy, void *stream) {
+    return guarded([&]() -> Status {
+        if (!x || !w || !y || !offsets) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        LinearBlocksCall c;
+        c.x = x;
+        c.w = w;
+        c.dtype = E_U8;
+        c.M = M;
+        c.N = N;
+        c.K = K;
+        c.ldx = ldx;
+        c.ldw = ldw;
+        c.offsets = offsets;
+        c.w_group = w_group;
+        c.xs = x_scale;
+        c.ld_xs = ld_xs;
+        c.ws = w_scale;
+        c.ld_ws = ld_ws;
+        c.ws_group = ws_group;
+        c.bias = bias;
+        c.y = y;
+        c.ldy = ldy;
+        return linear_blocks_entry(c, groups, y_dtype, accumulate, act, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -268,6 +268,50 @@ Status launch_convert(const float *src, void *dst, int64_t n, int mode, cudaStre
 
 int num_sms();
 
+// Block-scaled E4M3 operands (quantize.cu): q = e4m3(x / s), one scale s per block of block_rows
+// (1 or 128) x 128 elements, s the smallest power of two with max|x| / s <= 448 (at least 2^-126);
+// s and q are NaN for a block that holds an infinity or a NaN. x_dtype E_F32X, E_F16 or E_BF16.
+struct QuantizeCall {
+    const void *x = nullptr;
+    int x_dtype = E_BF16;
+    int64_t rows = 0, cols = 0, ldx = 0;
+    int block_rows = 1;
+    uint8_t *q = nullptr;
+    int64_t ldq = 0;
+    float *scale = nullptr;
+    int64_t ld_scale = 0;
+};
+Status launch_quantize_e4m3(const QuantizeCall &c, cudaStream_t stream);
+
+// Products over block-scaled E4M3 operands, and products grouped by expert (linear_blocks.cu):
+// y[r] (+)= act(x[r] W[e]^T + bias[e]) for the rows r of group e.
+struct LinearBlocksCall {
+    const void *x = nullptr, *w = nullptr;
+    int dtype = E_BF16;  // E_BF16, E_F16, or E_U8 = E4M3 with scales
+    int64_t M = 0, N = 0, K = 0, ldx = 0, ldw = 0;
+    // Groups: group e has rows [offsets[e], offsets[e + 1]) and the weight at w + e * w_group
+    // elements. offsets (device memory) may be null for one group of all rows.
+    const int32_t *offsets = nullptr;
+    int64_t groups = 1, w_group = 0;
+    // E_U8: x[r, k] stands for x * xs[r * ld_xs + k / 128] and w[e, n, k] for
+    // w * ws[e * ws_group + (n / 128) * ld_ws + k / 128].
+    const float *xs = nullptr, *ws = nullptr;
+    int64_t ld_xs = 0, ld_ws = 0, ws_group = 0;
+    const float *bias = nullptr;  // [groups, N] or null
+    void *y = nullptr;
+    int y_dtype = TSFM_DTYPE_BF16;  // tsfm_dtype
+    int64_t ldy = 0;
+    bool accumulate = false;  // y += (FP32 y); the activation then applies to the sum
+    int act = 0;              // 0 none, 1 relu, ACT_GLU (as LinearCall)
+    int *err = nullptr;
+};
+Status launch_linear_blocks(const LinearBlocksCall &c, cudaStream_t stream);
+
+// Tensor map over [d2, d1, d0] elements (d0 innermost; d2 = 0 for two dimensions), row stride ld1 and
+// block stride ld2 in elements, box (box0, box1, 1), 128-byte swizzle, zero fill outside.
+Status make_tmap_3d(void *map, const void *base, int dtype, int64_t d0, int64_t d1, int64_t d2, int64_t ld1, int64_t ld2,
+                    uint32_t box0, uint32_t box1);
+
 }  // namespace tsfm
 
 namespace tsfm {

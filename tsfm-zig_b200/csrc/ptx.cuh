@@ -28,6 +28,11 @@ enum : int {
     ERR_SITE_ATTN_SOFTMAX = 0x0203,
     ERR_SITE_ATTN_DRAIN = 0x0204,
     ERR_SITE_WAIT_TEST = 0x0301,
+    ERR_SITE_BLOCKS_PRODUCER = 0x0401,
+    ERR_SITE_BLOCKS_MMA_FULL = 0x0402,
+    ERR_SITE_BLOCKS_MMA_EMPTY = 0x0403,
+    ERR_SITE_BLOCKS_EPILOGUE = 0x0404,
+    ERR_SITE_BLOCKS_DRAIN = 0x0405,
 };
 
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s
@@ -179,6 +184,25 @@ __device__ __forceinline__ void tma_load_2d_pair(void *smem_dst, const CUtensorM
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(mbar_cluster_addr), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+// 3-D tiled loads (c0 = innermost, c1, c2), for one CTA and for one CTA of a pair; a box that runs
+// past the end of dimension 1 is zero-filled there.
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int32_t c0,
+                                            int32_t c1, int32_t c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorMap *map, uint32_t mbar_cluster_addr,
+                                                 int32_t c0, int32_t c1, int32_t c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(mbar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
 
