@@ -307,10 +307,10 @@ struct LinearBlocksCall {
 };
 Status launch_linear_blocks(const LinearBlocksCall &c, cudaStream_t stream);
 
-// Tensor map over [d2, d1, d0] elements (d0 innermost; d2 = 0 for two dimensions), row stride ld1 and
-// block stride ld2 in elements, box (box0, box1, 1), 128-byte swizzle, zero fill outside.
-Status make_tmap_3d(void *map, const void *base, int dtype, int64_t d0, int64_t d1, int64_t d2, int64_t ld1, int64_t ld2,
-                    uint32_t box0, uint32_t box1);
+// Tensor map of `rank` dimensions, innermost first: dims and strides in elements (strides[0] unused),
+// box extents, 128-byte swizzle, zero fill outside.
+Status make_tmap_nd(void *map, const void *base, int dtype, int rank, const int64_t *dims, const int64_t *strides,
+                    const uint32_t *box);
 
 }  // namespace tsfm
 

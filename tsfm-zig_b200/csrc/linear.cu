@@ -1042,22 +1042,29 @@ Status make_tmap_grouped_rows(void *map, const void *base, int dtype, int64_t wi
     return Status::ok();
 }
 
-Status make_tmap_3d(void *map, const void *base, int dtype, int64_t d0, int64_t d1, int64_t d2, int64_t ld1, int64_t ld2,
-                    uint32_t box0, uint32_t box1) {
+Status make_tmap_nd(void *map, const void *base, int dtype, int rank, const int64_t *dims, const int64_t *strides,
+                    const uint32_t *box) {
     if (!load_encode()) return Status::fail(TSFM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
     const int esz = dtype == E_F32 ? 4 : dtype == E_U8 ? 1 : 2;
     const CUtensorMapDataType dt = dtype == E_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == E_U8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : dtype == E_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    if ((reinterpret_cast<uintptr_t>(base) & 15) || ((ld1 * esz) & 15) || (d2 > 0 && ((ld2 * esz) & 15)))
-        return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: operand base and strides must be 16-byte aligned");
-    cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
-    cuuint64_t strides[2] = {(cuuint64_t)(ld1 * esz), (cuuint64_t)(ld2 * esz)};
-    cuuint32_t box[3] = {box0, box1, 1};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = g_encode(static_cast<CUtensorMap *>(map), dt, d2 > 0 ? 3 : 2, const_cast<void *>(base), dims, strides,
-                          box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    cuuint64_t d[5], st[4];
+    cuuint32_t bx[5], estr[5];
+    bool ok = (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+    for (int i = 0; i < rank; ++i) {
+        d[i] = (cuuint64_t)dims[i];
+        bx[i] = box[i];
+        estr[i] = 1;
+        if (i > 0) {
+            st[i - 1] = (cuuint64_t)(strides[i] * esz);
+            ok = ok && st[i - 1] % 16 == 0;
+        }
+    }
+    if (!ok) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: operand base and strides must be 16-byte aligned");
+    CUresult r = g_encode(static_cast<CUtensorMap *>(map), dt, (cuuint32_t)rank, const_cast<void *>(base), d, st, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return Status::fail(TSFM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
     return Status::ok();
 }

@@ -8,13 +8,24 @@
 // are added, scaled, into FP32 registers. 16-bit operands have no scales: their sums stay in tensor
 // memory over the whole of K.
 //
-// One CTA per SM walks tiles of 128 rows x BN columns (or a CTA pair, 256 x BN):
-//   warp 0     TMA producer: K-major tiles of x and W with the 128-byte swizzle into a ring of
-//              STAGES, 128 bytes of K a stage. W's tile comes as two boxes of BN / 2 rows, so that
-//              for gated pairs ([g | u] blocks of 256 rows) a tile holds g and u of the same columns.
-//   warp 1     tensor-memory allocation, MMA issue (one thread) into NBUF accumulators: one
-//              accumulator per block of K (E4M3) or per tile (16 bits).
-//   warps 2..  epilogue: a thread owns a row and BN (or BN / 2, with 8 warps) of its columns.
+// One CTA per SM walks tiles of 128 rows x BN columns, BN 64 or 128, or a CTA pair tiles of 256 x 256:
+//   warp 0      TMA producer (and warp 2, for alternate stages, below 256 columns): K-major tiles of x
+//               and W with the 128-byte swizzle into a ring of STAGES, 128 bytes of K a stage. For
+//               gated pairs ([g | u] blocks of 256 rows) W's box holds BN / 2 rows of each, so that
+//               a tile holds g and u of the same columns.
+//   warp 1      tensor-memory allocation, MMA issue (one lane) into accumulators in tensor memory:
+//               one per tile (16 bits, two in turn) or one per block of K (E4M3).
+//   warp 3      E4M3: the scales of the tile's rows and columns into a ring of shared memory, four
+//               blocks of K at a time, ahead of the tiles that need them.
+//   warps 4..   epilogue: a thread owns a row and 128 (below 256 columns: 64) of its columns. The
+//               finished sums pass through 4 KB of shared memory a warp, 32 columns at a time, to
+//               row-contiguous stores. That part is kept in small loops: unrolled over the outputs'
+//               types it outgrew the instruction cache, and every step of the kernel took three
+//               times as long.
+// E4M3 on 256 columns: each warpgroup of the epilogue has accumulators of its own (two of 128
+// columns), filled by MMAs of its half of the columns, so that handing one back and forth (MMA 256
+// cycles, commit and waits 300, loads 350) takes less than the 1024 cycles that the tensor cores
+// need for two blocks of K.
 // Rows of a group that end inside a tile: the tile's other rows hold whatever follows in x (or the
 // stage's old bytes), are computed and not stored.
 //
@@ -35,24 +46,35 @@ namespace {
 
 constexpr int kMaxGroups = 1024;  // two words of shared memory each
 
+// Blocks of K whose scales share a slot of the ring, and the slots.
+constexpr int kScaleQuad = 4, kScaleSlots = 4;
+constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2) * 4;  // [block of K][row], then [half tile][block of K]
+
 // KIND: element type of x and W (E_F16, E_BF16, E_U8 = E4M3).
-template <int KIND, int BN, bool PAIR>
+template <int KIND, int BN>
 struct BlkCfg {
+    static_assert(BN == 64 || BN == 128 || BN == 256, "tile widths");
     static constexpr bool F8 = KIND == E_U8;
-    static constexpr int EPI_WARPS = BN >= 128 ? 8 : 4;
-    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr bool PAIR = BN == 256;
+    static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;
+    static constexpr int THREADS = 128 + 32 * EPI_WARPS;
     static constexpr int TILE_M = PAIR ? 256 : 128;
-    static constexpr int A_BOX = BN >= 128 ? 128 : 32;  // rows of x per TMA box
+    static constexpr int A_BOX = BN == 256 ? 128 : 32;  // rows of x per TMA box
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // rows of W in this CTA's shared memory
     static constexpr int B_BYTES = B_ROWS * 128;
-    static constexpr int STAGES = BN == 64 ? 8 : BN == 256 && !PAIR ? 3 : 5;
-    static constexpr int NBUF = F8 ? (512 / BN > 8 ? 8 : 512 / BN) : 2;
+    static constexpr int STAGES = BN == 64 ? 8 : 5;
+    static constexpr int PRODUCERS = BN == 256 ? 1 : 2;
+    // Accumulators: NH column parts of BN / NH columns, NBUF of each.
+    static constexpr int NH = F8 && BN == 256 ? 2 : 1;
+    static constexpr int NBUF = !F8 || BN == 256 ? 2 : 512 / BN;
     static constexpr int TMEM_COLS = NBUF * BN;
     static constexpr int EPI_OFF = STAGES * (A_BYTES + B_BYTES);
-    static constexpr int BAR_OFF = EPI_OFF + EPI_WARPS * 4096;
+    static constexpr int SCALE_OFF = EPI_OFF + EPI_WARPS * 4096;
+    static constexpr int BAR_OFF = SCALE_OFF + (F8 ? kScaleSlots * kScaleSlotBytes : 0);
     static constexpr int GROUP_OFF = BAR_OFF + 512;
     static int smem(int64_t groups) { return 1024 + GROUP_OFF + 8 * (int)(groups + 1); }
+    static_assert((2 * STAGES + 2 * NH * NBUF + 2 * kScaleSlots + 2) * 8 <= 512, "barriers");
 };
 
 struct BlkArgs {
@@ -65,99 +87,96 @@ struct BlkArgs {
     const float *bias;
     void *y;
     int64_t ldy, ycols;
-    int y_dtype, accumulate, act, vec;
+    int y_dtype, accumulate, act;
+    int vec;       // y's base and row stride suit 4-element stores
+    int vec32;     // and 32-byte ones
+    int split;     // CTAs of a cluster that share a tile's K (1: none)
     int *err;
 };
 
-template <int DT>
-__device__ __forceinline__ uint32_t pack2_dt(float a, float b) {
-    return pack16<DT == TSFM_DTYPE_F16>(a, b);
-}
-
 __device__ __forceinline__ float silu_fast(float u) { return __fdividef(u, 1.0f + __expf(-u)); }
 
-// Stores (or adds) one 32-row x 32-column chunk of a warp: lane = row in, rows leave contiguous.
-// `box` is the warp's 4 KB of shared memory; row0 the chunk's first row, rows its valid rows.
-__device__ __forceinline__ void store_chunk32(const BlkArgs &a, uint8_t *box, int lane, int64_t row0, int rows,
-                                              int64_t col0, const float (&v)[32]) {
-    const bool f32 = a.y_dtype == TSFM_DTYPE_F32;
-    const int64_t left = a.ycols - col0;
-    if (left <= 0 || rows <= 0) return;  // the same for the whole warp
-    __syncwarp();
-    if (f32) {
+// Bias of four consecutive columns of group e (zero past N).
+__device__ __forceinline__ void bias_quad(const BlkArgs &a, int e, int64_t col, float (&b)[4]) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4 *>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    } else {
-        const bool h = a.y_dtype == TSFM_DTYPE_F16;
+    for (int j = 0; j < 4; ++j) b[j] = a.bias && col + j < a.N ? __ldg(a.bias + e * a.N + col + j) : 0.0f;
+}
+
+// y of four consecutive columns of one row (the last columns of a row: fewer): adds to it or not,
+// activates and stores.
+__device__ __forceinline__ void store_quad(const BlkArgs &a, int64_t row, int64_t col, float (&v)[4]) {
+    const int64_t at = row * a.ldy + col;
+    const int n = (int)min((int64_t)4, a.ycols - col);
+    if (a.accumulate) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint4 p;
-            p.x = h ? pack16<true>(v[8 * q], v[8 * q + 1]) : pack16<false>(v[8 * q], v[8 * q + 1]);
-            p.y = h ? pack16<true>(v[8 * q + 2], v[8 * q + 3]) : pack16<false>(v[8 * q + 2], v[8 * q + 3]);
-            p.z = h ? pack16<true>(v[8 * q + 4], v[8 * q + 5]) : pack16<false>(v[8 * q + 4], v[8 * q + 5]);
-            p.w = h ? pack16<true>(v[8 * q + 6], v[8 * q + 7]) : pack16<false>(v[8 * q + 6], v[8 * q + 7]);
-            *reinterpret_cast<uint4 *>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = p;
-        }
+        for (int j = 0; j < 4; ++j)
+            if (j < n) v[j] += static_cast<const float *>(a.y)[at + j];
     }
-    __syncwarp();
-    if (a.vec && left >= 32) {
-        if (f32) {
+    if (a.act == 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3), q = lane & 7;
-                if (r < rows) {
-                    float4 t = *reinterpret_cast<const float4 *>(box + r * 128 + ((q ^ (r & 7)) << 4));
-                    float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(a.y) + (row0 + r) * a.ldy + col0) + q;
-                    if (a.accumulate) {
-                        const float4 old = *o;
-                        t.x += old.x, t.y += old.y, t.z += old.z, t.w += old.w;
-                        if (a.act == 1) t = make_float4(fmaxf(t.x, 0.f), fmaxf(t.y, 0.f), fmaxf(t.z, 0.f), fmaxf(t.w, 0.f));
-                    }
-                    *o = t;
-                }
-            }
+        for (int j = 0; j < 4; ++j) v[j] = fmaxf(v[j], 0.0f);
+    }
+    if (a.y_dtype == TSFM_DTYPE_F32) {
+        float *o = static_cast<float *>(a.y) + at;
+        if (a.vec && n == 4) {
+            *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 8 * i + (lane >> 2), q = lane & 3;
-                if (r < rows)
-                    reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.y) + (row0 + r) * a.ldy + col0)[q] =
-                        *reinterpret_cast<const uint4 *>(box + r * 128 + ((q ^ (r & 7)) << 4));
-            }
+            for (int j = 0; j < 4; ++j)
+                if (j < n) o[j] = v[j];
         }
-    } else if (lane < left) {
-        // A column tail or an unaligned y: one element per lane.
-        for (int r = 0; r < rows; ++r) {
-            if (f32) {
-                float t = *reinterpret_cast<const float *>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                float *o = static_cast<float *>(a.y) + (row0 + r) * a.ldy + col0 + lane;
-                if (a.accumulate) {
-                    t += *o;
-                    if (a.act == 1) t = fmaxf(t, 0.0f);
-                }
-                *o = t;
-            } else {
-                static_cast<uint16_t *>(a.y)[(row0 + r) * a.ldy + col0 + lane] = *reinterpret_cast<const uint16_t *>(
-                    box + r * 128 + (((lane >> 3) ^ (r & 7)) << 4) + (lane & 7) * 2);
-            }
+    } else {
+        const bool h = a.y_dtype == TSFM_DTYPE_F16;
+        const uint32_t w[2] = {h ? pack16<true>(v[0], v[1]) : pack16<false>(v[0], v[1]),
+                               h ? pack16<true>(v[2], v[3]) : pack16<false>(v[2], v[3])};
+        uint16_t *o = static_cast<uint16_t *>(a.y) + at;
+        if (a.vec && n == 4) {
+            *reinterpret_cast<uint2 *>(o) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < n) o[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
         }
     }
 }
 
-template <int KIND, int BN, bool PAIR>
-__global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
-    linear_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, BlkArgs a) {
-    using C = BlkCfg<KIND, BN, PAIR>;
-    constexpr bool F8 = C::F8;
-    constexpr int STAGES = C::STAGES, NBUF = C::NBUF;
+// 32 consecutive values of one row, 32 bytes a store; o 32-byte aligned.
+template <int DT>
+__device__ __forceinline__ void store_sectors(void *o, const float (&v)[32]) {
+    if constexpr (DT == TSFM_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(v) + 8 * i;
+            st_global_v8(static_cast<float *>(o) + 8 * i, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = pack16<DT == TSFM_DTYPE_F16>(v[16 * i + 2 * j], v[16 * i + 2 * j + 1]);
+            st_global_v8(static_cast<uint16_t *>(o) + 16 * i, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+        }
+    }
+}
+
+template <int KIND, int BN>
+__global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
+    linear_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         BlkArgs a) {
+    using C = BlkCfg<KIND, BN>;
+    constexpr bool F8 = C::F8, PAIR = C::PAIR;
+    constexpr int STAGES = C::STAGES, NBUF = C::NBUF, NH = C::NH;
     constexpr int BK = F8 ? 128 : 64;  // elements of K per stage
-    constexpr uint32_t IDESC = idesc_f32acc(KIND == E_BF16 ? 1u : 0u, C::TILE_M, BN);
-    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
-    const bool leader = rank == 0;
-    const int64_t unit = PAIR ? (int64_t)(blockIdx.x >> 1) : (int64_t)blockIdx.x;
-    const int64_t units = PAIR ? (int64_t)(gridDim.x >> 1) : (int64_t)gridDim.x;
+    // 384 threads launch with 168 registers each; the epilogue's two warpgroups (128 sums and 64 loaded
+    // values a thread) take them from the first one: 64,512 = 128 x 56 + 256 x 224.
+    constexpr bool SPLIT_REGS = F8 && BN == 256;
+    constexpr uint32_t IDESC = idesc_f32acc(KIND == E_BF16 ? 1u : 0u, C::TILE_M, BN / NH);
+    const int cta_split = BN == 256 ? 1 : a.split;  // CTAs that share a tile's K
+    const int cta = PAIR ? 2 : cta_split;           // CTAs of a cluster
+    const uint32_t rank = cta > 1 ? cluster_ctarank() : 0u;
+    const bool leader = !PAIR || rank == 0;
+    const int unit = (int)blockIdx.x / cta, units = (int)gridDim.x / cta;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -165,9 +184,11 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
     uint8_t *sB = smem + STAGES * C::A_BYTES;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);
     uint64_t *empty = full + STAGES;
-    uint64_t *pfull = empty + STAGES;
-    uint64_t *pempty = pfull + NBUF;
-    uint64_t *drain = pempty + NBUF;
+    uint64_t *pfull = empty + STAGES;       // accumulators, [NH][NBUF]
+    uint64_t *pempty = pfull + NH * NBUF;
+    uint64_t *sfull = pempty + NH * NBUF;   // scales
+    uint64_t *sempty = sfull + kScaleSlots;
+    uint64_t *drain = sempty + kScaleSlots;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *g_row = reinterpret_cast<int *>(smem + C::GROUP_OFF);  // group e has rows [g_row[e], g_row[e + 1])
@@ -175,14 +196,18 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (threadIdx.x == 32) {
+    if (threadIdx.x == 64) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int i = 0; i < NBUF; ++i) {
+        for (int i = 0; i < NH * NBUF; ++i) {
             mbar_init(&pfull[i], 1);
-            mbar_init(&pempty[i], (PAIR ? 2 : 1) * C::EPI_WARPS);  // one arrival per epilogue warp
+            mbar_init(&pempty[i], (PAIR ? 2 : 1) * C::EPI_WARPS / NH);  // one arrival per epilogue warp
+        }
+        for (int i = 0; i < kScaleSlots; ++i) {
+            mbar_init(&sfull[i], 32);
+            mbar_init(&sempty[i], C::EPI_WARPS);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -241,13 +266,14 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
 
     struct Tile {
         int e, row0, row_end;  // group, first row of this CTA's 128 rows, end of the group
-        int b0, b1;            // first W row of the tile's two boxes
-        int ocol0, ocol1;      // the boxes' output columns
+        int b0, b1;            // W rows of the tile's first and second BN / 2 columns
+        int ocol;              // first output column
     };
-    const int64_t tiles = (int64_t)g_tile[a.groups] * a.n_tiles;
-    auto tile_at = [&](int64_t t) {
+    const int tiles = g_tile[a.groups] * a.n_tiles;  // the host has checked that this fits
+    const bool glu = a.act == ACT_GLU;
+    auto tile_at = [&](int t) {
         Tile r;
-        const int mt = (int)(t / a.n_tiles), nt = (int)(t - (int64_t)mt * a.n_tiles);
+        const int mt = t / a.n_tiles, nt = t - mt * a.n_tiles;
         int lo = 0, hi = a.groups - 1;  // the last e with g_tile[e] <= mt
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -257,53 +283,70 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
                 hi = mid - 1;
         }
         r.e = lo;
-        r.row0 = g_row[lo] + (mt - g_tile[lo]) * C::TILE_M + (int)rank * 128;
+        r.row0 = g_row[lo] + (mt - g_tile[lo]) * C::TILE_M + (PAIR ? (int)rank * 128 : 0);
         r.row_end = g_row[lo + 1];
-        if (a.act == ACT_GLU) {
-            const int c = nt * (BN / 2);
-            r.b0 = (c >> 7) * 256 + (c & 127);
+        if (glu) {
+            r.ocol = nt * (BN / 2);
+            r.b0 = (r.ocol >> 7) * 256 + (r.ocol & 127);
             r.b1 = r.b0 + 128;
-            r.ocol0 = r.ocol1 = c;
         } else {
-            r.ocol0 = r.b0 = nt * BN;
-            r.ocol1 = r.b1 = r.b0 + BN / 2;
+            r.ocol = r.b0 = nt * BN;
+            r.b1 = r.b0 + BN / 2;
         }
         return r;
     };
-    auto slabs = [&](int row0, int row_end) {  // boxes of x that hold rows of the tile
-        return min(128 / C::A_BOX, max(0, (row_end - row0 + C::A_BOX - 1) / C::A_BOX));
+    // This CTA's blocks of K.
+    const int kb0 = cta_split > 1 ? (int)((int64_t)a.num_k * rank / cta) : 0;
+    const int kb1 = cta_split > 1 ? (int)((int64_t)a.num_k * (rank + 1) / cta) : a.num_k;
+    const int kbn = kb1 - kb0;
+    // Waits on barriers that hand over stages and accumulators. In a pair the other CTA's arrivals
+    // stand for completed copies, MMAs and tensor-memory loads, none of them accesses that an
+    // acquire at cluster scope would order: the plain form does, and the other costs over 1000 cycles.
+    // Every role's loop is warp-uniform, with one elected lane that issues.
+    auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        return mbar_wait_warp(bar, parity, abort_flag, a.err, site);
     };
 
-    if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
+    if (warp < 4) {
+        if constexpr (SPLIT_REGS) regs_dec<56>();
+        if (warp == 0 || (C::PRODUCERS == 2 && warp == 2)) {
+            // Producers: of two, stage use number i (over all tiles) belongs to warp 2 (i % 2).
+            const bool el = elect_one();
+            const int mine = warp >> 1;
+            int s = mine % STAGES, turn = 0;  // turn: parity of i for the next block of K
             uint32_t ph = 0, issued = 0, issued_ph = 0;
             bool ok = true;
-            for (int64_t t = unit; t < tiles && ok; t += units) {
+            for (int t = unit; t < tiles && ok; t += units) {
                 const Tile tl = tile_at(t);
-                const int na = PAIR ? 1 : slabs(tl.row0, tl.row_end);
-                for (int kb = 0; kb < a.num_k; ++kb) {
-                    ok = PAIR ? mbar_wait_cl(&empty[s], ph ^ 1u, abort_flag, a.err, ERR_SITE_BLOCKS_PRODUCER)
-                              : mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, ERR_SITE_BLOCKS_PRODUCER);
+                const int na = min(128 / C::A_BOX, max(0, (tl.row_end - tl.row0 + C::A_BOX - 1) / C::A_BOX));
+                const int c1 = glu ? tl.ocol & 127 : tl.b0, c3 = glu ? tl.ocol >> 7 : 0;
+                for (int kb = kb0; kb < kb1; ++kb, turn ^= C::PRODUCERS - 1) {
+                    if (turn != mine) continue;
+                    ok = wait(&empty[s], ph ^ 1u, ERR_SITE_BLOCKS_PRODUCER);
                     if (!ok) break;
                     const int32_t kc = kb * BK;
-                    if constexpr (PAIR) {
-                        // Each CTA loads its 128 rows of x and one of W's two boxes.
-                        if (leader) mbar_arrive_expect_tx(&full[s], 2 * (C::A_BYTES + C::B_BYTES));
-                        const uint32_t fb = mapa_shared(&full[s], 0);
-                        tma_load_2d_pair(sA + s * C::A_BYTES, &tmA, fb, kc, tl.row0);
-                        tma_load_3d_pair(sB + s * C::B_BYTES, &tmB, fb, kc, leader ? tl.b0 : tl.b1, tl.e);
-                    } else {
-                        mbar_arrive_expect_tx(&full[s], na * C::A_BOX * 128 + C::B_BYTES);
-                        for (int i = 0; i < na; ++i)
-                            tma_load_2d(sA + s * C::A_BYTES + i * C::A_BOX * 128, &tmA, &full[s], kc, tl.row0 + i * C::A_BOX);
-                        tma_load_3d(sB + s * C::B_BYTES, &tmB, &full[s], kc, tl.b0, tl.e);
-                        tma_load_3d(sB + s * C::B_BYTES + C::B_BYTES / 2, &tmB, &full[s], kc, tl.b1, tl.e);
+                    if (el) {
+                        if constexpr (PAIR) {
+                            // Each CTA loads its 128 rows of x and half of W's rows.
+                            if (leader) mbar_arrive_expect_tx(&full[s], 2 * (C::A_BYTES + C::B_BYTES));
+                            const uint32_t fb = mapa_shared(&full[s], 0);
+                            tma_load_2d_pair(sA + s * C::A_BYTES, &tmA, fb, kc, tl.row0);
+                            tma_load_5d_pair(sB + s * C::B_BYTES, &tmB, fb, kc, glu ? 0 : c1 + (int)rank * (BN / 2),
+                                             glu ? (int)rank : 0, c3, tl.e);
+                        } else {
+                            mbar_arrive_expect_tx(&full[s], na * C::A_BOX * 128 + C::B_BYTES);
+                            for (int i = 0; i < na; ++i)
+                                tma_load_2d(sA + s * C::A_BYTES + i * C::A_BOX * 128, &tmA, &full[s], kc,
+                                            tl.row0 + i * C::A_BOX);
+                            tma_load_5d(sB + s * C::B_BYTES, &tmB, &full[s], kc, c1, 0, c3, tl.e);
+                        }
                     }
+                    __syncwarp();
                     issued |= 1u << s;
                     issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
-                    if (++s == STAGES) {
-                        s = 0;
+                    s += C::PRODUCERS;
+                    if (s >= STAGES) {
+                        s -= STAGES;
                         ph ^= 1u;
                     }
                 }
@@ -318,191 +361,293 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
                 } else {
                     for (int i = 0; i < STAGES; ++i) {
                         if (!((issued >> i) & 1u)) continue;
-                        while (!mbar_try_wait_cl(&full[i], (issued_ph >> i) & 1u) && globaltimer_ns() - t0 < 100000000ull) {
+                        while (!mbar_try_wait(&full[i], (issued_ph >> i) & 1u) && globaltimer_ns() - t0 < 100000000ull) {
                         }
                     }
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && leader) {
-            int s = 0, buf = 0;
-            uint32_t ph = 0, bph = 0;
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
-                return PAIR ? mbar_wait_cl(bar, parity, abort_flag, a.err, site) : mbar_wait(bar, parity, abort_flag, a.err, site);
-            };
-            auto commit = [&](uint64_t *bar) {
-                if constexpr (PAIR) {
-                    mma_commit_pair(mapa_shared(bar, 0));
-                    mma_commit_pair(mapa_shared(bar, 1));
-                } else {
-                    mma_commit(bar);
-                }
-            };
-            for (int64_t t = unit; t < tiles && ok; t += units) {
-                for (int kb = 0; kb < a.num_k; ++kb) {
-                    if (F8 || kb == 0) {
-                        ok = wait(&pempty[buf], bph ^ 1u, ERR_SITE_BLOCKS_MMA_EMPTY);
+        } else if (warp == 1) {
+            if (leader) {
+                const bool el = elect_one();
+                int s = 0, buf = 0;
+                uint32_t ph = 0, bph = 0;
+                bool ok = true;
+                const uint64_t ad0 = sdesc_k128(sA), bd0 = sdesc_k128(sB);
+                auto commit = [&](uint64_t *bar) {
+                    if constexpr (PAIR) {
+                        mma_commit_pair(mapa_shared(bar, 0));
+                        mma_commit_pair(mapa_shared(bar, 1));
+                    } else {
+                        mma_commit(bar);
+                    }
+                };
+                for (int t = unit; t < tiles && ok; t += units) {
+                    for (int kb = 0; kb < kbn; ++kb) {
+                        ok = wait(&full[s], ph, ERR_SITE_BLOCKS_MMA_FULL);
                         if (!ok) break;
-                    }
-                    ok = wait(&full[s], ph, ERR_SITE_BLOCKS_MMA_FULL);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t d = tmem_base + (uint32_t)(buf * BN);
-                    const uint64_t ad = sdesc_k128(sA + s * C::A_BYTES), bd = sdesc_k128(sB + s * C::B_BYTES);
+                        const uint64_t ad = ad0 + (uint64_t)(s * (C::A_BYTES >> 4)), bd = bd0 + (uint64_t)(s * (C::B_BYTES >> 4));
+                        const bool last = F8 || kb == kbn - 1;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint32_t accum = F8 ? kk != 0 : (kb | kk) != 0;
-                        if constexpr (F8) {
-                            if constexpr (PAIR)
-                                mma_f8kind_pair(d, ad + 2 * kk, bd + 2 * kk, IDESC, accum);
-                            else
-                                mma_f8kind(d, ad + 2 * kk, bd + 2 * kk, IDESC, accum);
-                        } else if constexpr (PAIR) {
-                            mma_f16kind_pair(d, ad + 2 * kk, bd + 2 * kk, IDESC, accum);
-                        } else {
-                            mma_f16kind(d, ad + 2 * kk, bd + 2 * kk, IDESC, accum);
+                        for (int h = 0; h < NH; ++h) {
+                            const int acc = h * NBUF + buf;
+                            if (F8 || kb == 0) {
+                                ok = wait(&pempty[acc], bph ^ 1u, ERR_SITE_BLOCKS_MMA_EMPTY);
+                                if (!ok) break;
+                            }
+                            tc_fence_after();
+                            const uint32_t d = tmem_base + (uint32_t)(acc * (BN / NH));
+                            const uint64_t bh = bd + (uint64_t)(h * (C::B_BYTES / NH >> 4));
+                            if (el) {
+#pragma unroll
+                                for (int kk = 0; kk < 4; ++kk) {
+                                    const uint32_t accum = F8 ? kk != 0 : (kb | kk) != 0;
+                                    if constexpr (F8) {
+                                        if constexpr (PAIR)
+                                            mma_f8kind_pair(d, ad + 2 * kk, bh + 2 * kk, IDESC, accum);
+                                        else
+                                            mma_f8kind(d, ad + 2 * kk, bh + 2 * kk, IDESC, accum);
+                                    } else if constexpr (PAIR) {
+                                        mma_f16kind_pair(d, ad + 2 * kk, bh + 2 * kk, IDESC, accum);
+                                    } else {
+                                        mma_f16kind(d, ad + 2 * kk, bh + 2 * kk, IDESC, accum);
+                                    }
+                                }
+                                if (last) commit(&pfull[acc]);
+                                if (h == NH - 1) commit(&empty[s]);
+                            }
+                            __syncwarp();
                         }
-                    }
-                    commit(&empty[s]);
-                    if (F8 || kb == a.num_k - 1) {
-                        commit(&pfull[buf]);
-                        if (++buf == NBUF) {
+                        if (!ok) break;
+                        if (last && ++buf == NBUF) {
                             buf = 0;
                             bph ^= 1u;
                         }
+                        if (++s == STAGES) {
+                            s = 0;
+                            ph ^= 1u;
+                        }
                     }
-                    if (++s == STAGES) {
-                        s = 0;
+                }
+                // All MMAs issued by this warp have completed once `drain` fires; the tensor memory can
+                // then be released safely even on the abort path.
+                if (el) {
+                    if constexpr (PAIR)
+                        mma_commit_pair(mapa_shared(drain, 0));
+                    else
+                        mma_commit(drain);
+                    const unsigned long long t0 = globaltimer_ns();
+                    while (!mbar_try_wait(drain, 0)) {
+                        if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+                            if (a.err) atomicCAS(a.err, 0, ERR_SITE_BLOCKS_DRAIN);
+                            break;
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+        } else if (F8 && warp == 3) {
+            // Scales: slot = xs[4][128] then ws[2][4] (the half tiles' column blocks), by asynchronous
+            // copies; entries past this CTA's last block of K are not read.
+            int slot = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = unit; t < tiles && ok; t += units) {
+                const Tile tl = tile_at(t);
+                const float *xs = a.xs + (int64_t)tl.row0 * a.ld_xs;
+                const int last = tl.row_end - 1 - tl.row0;  // rows past the group's end repeat its last
+                const int nb = min((lane & 4 ? tl.b1 : tl.b0) >> 7, a.ws_blocks - 1);
+                const float *ws = a.ws + tl.e * a.ws_group + (int64_t)nb * a.ld_ws + (lane & 3);
+                for (int kb = kb0; kb < kb1; kb += kScaleQuad) {
+                    ok = wait(&sempty[slot], ph ^ 1u, ERR_SITE_BLOCKS_PRODUCER);
+                    if (!ok) break;
+                    uint8_t *d = smem + C::SCALE_OFF + slot * kScaleSlotBytes;
+                    const int n = min(kScaleQuad, kb1 - kb);
+                    for (int r = lane; r < 128; r += 32) {
+                        const float *src = xs + (int64_t)min(r, last) * a.ld_xs + kb;
+                        for (int j = 0; j < n; ++j) cp_async_4(d + j * 512 + r * 4, src + j);
+                    }
+                    if (lane < 8 && (lane & 3) < n) cp_async_4(d + 2048 + lane * 4, ws + kb);
+                    cp_async_arrive(&sfull[slot]);
+                    if (++slot == kScaleSlots) {
+                        slot = 0;
                         ph ^= 1u;
                     }
                 }
             }
-            if constexpr (PAIR)
-                mma_commit_pair(mapa_shared(drain, 0));
-            else
-                mma_commit(drain);
-            const unsigned long long t0 = globaltimer_ns();
-            while (!mbar_try_wait(drain, 0)) {
-                if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
-                    if (a.err) atomicCAS(a.err, 0, ERR_SITE_BLOCKS_DRAIN);
-                    break;
-                }
-            }
+            cp_async_wait_all();
         }
     } else {
-        constexpr int PARTS = C::EPI_WARPS / 4;         // warps that share a row's columns
-        constexpr int CPH = BN / 2 / PARTS / 32;        // 32-column chunks per thread of each box
-        const int ew = warp - 2;
-        const int eg = warp & 3, part = ew >> 2;        // tensor-memory lanes [32 eg, 32 eg + 32)
-        uint8_t *box = smem + C::EPI_OFF + ew * 4096;
-        int buf = 0;
-        uint32_t bph = 0;
+        if constexpr (SPLIT_REGS) regs_inc<224>();
+        constexpr int PARTS = C::EPI_WARPS / 4;  // warps that share a row's columns
+        constexpr int CH = BN / PARTS / 32;      // 32-column chunks per thread
+        constexpr int CPH = CH / 2;              // of each half of the tile
+        const int ew = warp - 4;
+        const int eg = warp & 3, part = ew >> 2;  // tensor-memory lanes [32 eg, 32 eg + 32)
+        const int half = NH == 2 ? part : 0;      // this warp's accumulators
+        float4 *box = reinterpret_cast<float4 *>(smem + C::EPI_OFF + ew * 4096);
+        int buf = 0, slot = 0;
+        uint32_t bph = 0, sph = 0;
         bool ok = true;
-        auto wait = [&]() {
-            const bool got = PAIR ? mbar_wait_cl(&pfull[buf], bph, abort_flag, a.err, ERR_SITE_BLOCKS_EPILOGUE)
-                                  : mbar_wait(&pfull[buf], bph, abort_flag, a.err, ERR_SITE_BLOCKS_EPILOGUE);
-            return __all_sync(0xffffffffu, got) != 0;
-        };
+        auto wait_epi = [&](uint64_t *bar, uint32_t parity) { return wait(bar, parity, ERR_SITE_BLOCKS_EPILOGUE); };
+        const uint32_t handback = PAIR ? mapa_shared(&pempty[half * NBUF], 0) : 0u;  // the MMA-issuing CTA's barriers
         auto release = [&]() {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 if constexpr (PAIR)
-                    mbar_arrive_cluster(mapa_shared(&pempty[buf], 0));
+                    mbar_arrive_remote(handback + 8 * buf);
                 else
-                    mbar_arrive(&pempty[buf]);
+                    mbar_arrive(&pempty[half * NBUF + buf]);
             }
             if (++buf == NBUF) {
                 buf = 0;
                 bph ^= 1u;
             }
         };
-        for (int64_t t = unit; t < tiles && ok; t += units) {
-            const Tile tl = tile_at(t);
-            const int wrow0 = tl.row0 + eg * 32;
-            const int wrows = min(32, tl.row_end - wrow0);  // this warp's valid rows (may be <= 0)
-            // Chunk c of this thread: columns [off(c), off(c) + 32) of the tile's accumulator; chunks
-            // [0, CPH) belong to the first box, [CPH, 2 CPH) to the second.
-            auto off = [&](int c) { return (c / CPH) * (BN / 2) + (part * CPH + c % CPH) * 32; };
-            float acc[F8 ? 2 * CPH * 32 : 32];
+        // Chunk c of this thread: 32 columns of the accumulator from acol(c), y's columns from ycol(c).
+        // Gated pairs: chunk c < CPH is g's, chunk c + CPH the same columns of u.
+        auto acol = [&](int c) { return NH == 2 ? c * 32 : (c / CPH) * (BN / 2) + (part * CPH + c % CPH) * 32; };
+        auto ycol = [&](const Tile &tl, int c) { return (c < CPH ? tl.ocol : tl.b1) + (part * CPH + c % CPH) * 32; };
+        // The scales of the next block of K (over all tiles): the row's times each half's.
+        float s0 = 0.0f, s1 = 0.0f;
+        const uint32_t scales = smem_u32(smem) + C::SCALE_OFF;
+        auto next_scales = [&](int kb) {
+            const int j = kb & (kScaleQuad - 1);
+            // (A wait that gave up has raised the abort flag: the next accumulator's ends the loops.)
+            if (j == 0) wait_epi(&sfull[slot], sph);
+            const uint32_t sc = scales + slot * kScaleSlotBytes;
+            const float sx = ld_shared_f32(sc + j * 512 + (eg * 32 + lane) * 4);
+            s0 = sx * ld_shared_f32(sc + 2048 + j * 4);
+            s1 = sx * ld_shared_f32(sc + 2048 + 16 + j * 4);
+            if (j == kScaleQuad - 1 || kb == kbn - 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sempty[slot]);
+                if (++slot == kScaleSlots) {
+                    slot = 0;
+                    sph ^= 1u;
+                }
+            }
+        };
+        if (F8 && unit < tiles) next_scales(0);
+        for (int t = unit; t < tiles && ok; t += units) {
+            float2 acc[F8 ? CH : 1][16];
             uint32_t tbase = 0;
             if constexpr (F8) {
 #pragma unroll
-                for (int i = 0; i < 2 * CPH * 32; ++i) acc[i] = 0.0f;
-                const float *xs = a.xs + (int64_t)min(wrow0 + lane, tl.row_end - 1) * a.ld_xs;
-                const float *ws0 = a.ws + tl.e * a.ws_group + (int64_t)min(tl.b0 >> 7, a.ws_blocks - 1) * a.ld_ws;
-                const float *ws1 = a.ws + tl.e * a.ws_group + (int64_t)min(tl.b1 >> 7, a.ws_blocks - 1) * a.ld_ws;
-                float sx = __ldg(xs), w0 = __ldg(ws0), w1 = __ldg(ws1);
-                for (int kb = 0; kb < a.num_k; ++kb) {
-                    const float s0 = sx * w0, s1 = sx * w1;
-                    if (kb + 1 < a.num_k) {
-                        sx = __ldg(xs + kb + 1);
-                        w0 = __ldg(ws0 + kb + 1);
-                        w1 = __ldg(ws1 + kb + 1);
-                    }
-                    ok = wait();
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[c][j] = make_float2(0.0f, 0.0f);
+                for (int kb = 0; kb < kbn; ++kb) {
+                    ok = wait_epi(&pfull[half * NBUF + buf], bph);
                     if (!ok) break;
                     tc_fence_after();
-                    if (wrows > 0) {
-                        tbase = tmem_base + ((uint32_t)(eg * 32) << 16) + (uint32_t)(buf * BN);
+                    tbase = tmem_base + ((uint32_t)(eg * 32) << 16) + (uint32_t)((half * NBUF + buf) * (BN / NH));
+                    // The accumulator is handed back, and the next scales are read, before the last additions.
 #pragma unroll
-                        for (int c = 0; c < 2 * CPH; ++c) {
-                            float p[32];
-                            tmem_ld32(tbase + off(c), p);
-                            tmem_wait_ld();
-                            const float sc = c < CPH ? s0 : s1;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(p[j], sc, acc[c * 32 + j]);
+                    for (int c = 0; c < CH; c += 2) {
+                        float p[2][32];
+                        tmem_ld32f(tbase + acol(c), p[0]);
+                        tmem_ld32f(tbase + acol(c + 1), p[1]);
+                        tmem_wait_ld();
+                        const float2 sa = c < CPH ? make_float2(s0, s0) : make_float2(s1, s1);
+                        const float2 sb = c + 1 < CPH ? make_float2(s0, s0) : make_float2(s1, s1);
+                        if (c + 2 == CH) {
+                            release();
+                            if (kb + 1 < kbn || t + units < tiles) next_scales(kb + 1 < kbn ? kb + 1 : 0);
                         }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c][j], make_float2(p[0][2 * j], p[0][2 * j + 1]), sa);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c + 1][j], make_float2(p[1][2 * j], p[1][2 * j + 1]), sb);
                     }
-                    release();
                 }
                 if (!ok) break;
             } else {
-                ok = wait();
+                ok = wait_epi(&pfull[buf], bph);
                 if (!ok) break;
                 tc_fence_after();
                 tbase = tmem_base + ((uint32_t)(eg * 32) << 16) + (uint32_t)(buf * BN);
             }
+            const Tile tl = tile_at(t);
+            const int wrow0 = tl.row0 + eg * 32;
+            const int wrows = min(32, tl.row_end - wrow0);  // this warp's valid rows (may be <= 0)
             auto chunk = [&](int c, float (&v)[32]) {
                 if constexpr (F8) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = acc[c * 32 + j];
+                    for (int j = 0; j < 16; ++j) v[2 * j] = acc[c][j].x, v[2 * j + 1] = acc[c][j].y;
                 } else {
-                    tmem_ld32(tbase + off(c), v);
+                    tmem_ld32f(tbase + acol(c), v);
                     tmem_wait_ld();
                 }
             };
-            if (wrows > 0) {
-                if (a.act == ACT_GLU) {
+            // v to shared memory: float4 q of this thread's row at to[q ^ (lane % 8)].
+            auto dump = [&](const float (&v)[32], float4 *to) {
 #pragma unroll
-                    for (int c = 0; c < CPH; ++c) {
-                        float g[32], u[32];
-                        chunk(c, g);
-                        chunk(CPH + c, u);
+                for (int q = 0; q < 8; ++q)
+                    to[q ^ (lane & 7)] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            };
+            if (wrows > 0 && cta_split > 1) {
+                // A share of K: the sums go to shared memory (the stages', which are all used up), row r at
+                // float4 r * BN / 4, its chunks in order.
+                float4 *to = reinterpret_cast<float4 *>(smem) + (eg * 32 + lane) * (BN / 4);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) g[j] *= silu_fast(u[j]);
-                        store_chunk32(a, box, lane, wrow0, wrows, tl.ocol0 + off(c), g);
-                    }
-                } else {
+                for (int c = 0; c < CH; ++c) {
+                    float v[32];
+                    chunk(c, v);
+                    dump(v, to + acol(c) / 4);
+                }
+            } else if (wrows > 0) {
 #pragma unroll
-                    for (int c = 0; c < 2 * CPH; ++c) {
-                        float v[32];
-                        chunk(c, v);
-                        const int64_t col0 = (int64_t)tl.b0 + off(c);
-                        if (a.bias) {
-                            const float *b = a.bias + tl.e * a.N + col0;
+                for (int c = 0; c < CH; ++c) {
+                    if (glu && c >= CPH) break;
+                    const int col0 = ycol(tl, c);
+                    float v[32];
+                    chunk(c, v);
+                    if (glu) {
+                        float u[32];
+                        chunk((c + CPH) % CH, u);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] *= silu_fast(u[j]);
+                    } else if (a.bias) {
+                        const float *b = a.bias + tl.e * a.N + col0;
+                        if (col0 + 32 <= a.N) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] += __ldg(b + j);
+                        } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 if (col0 + j < a.N) v[j] += __ldg(b + j);
                         }
-                        if (a.act == 1 && !a.accumulate) {
+                    }
+                    if (a.vec32 && col0 + 32 <= a.ycols && !a.accumulate) {
+                        // A thread's 32 columns are whole 32-byte sectors of its row.
+                        if (a.act == 1) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = fmaxf(v[j], 0.0f);
                         }
-                        store_chunk32(a, box, lane, wrow0, wrows, col0, v);
+                        char *o = static_cast<char *>(a.y) + ((wrow0 + lane) * a.ldy + col0) * (a.y_dtype == TSFM_DTYPE_F32 ? 4 : 2);
+                        if (lane < wrows) {
+                            if (a.y_dtype == TSFM_DTYPE_F32)
+                                store_sectors<TSFM_DTYPE_F32>(o, v);
+                            else if (a.y_dtype == TSFM_DTYPE_F16)
+                                store_sectors<TSFM_DTYPE_F16>(o, v);
+                            else
+                                store_sectors<TSFM_DTYPE_BF16>(o, v);
+                        }
+                    } else {
+                        // Through shared memory to row-contiguous stores of whatever alignment.
+                        __syncwarp();
+                        dump(v, box + lane * 8);
+                        __syncwarp();
+                        const int q = lane & 7;
+                        if (col0 + 4 * q < a.ycols) {
+#pragma unroll 1
+                            for (int r = lane >> 3; r < wrows; r += 4) {
+                                const float4 f = box[r * 8 + (q ^ (r & 7))];
+                                float w[4] = {f.x, f.y, f.z, f.w};
+                                store_quad(a, wrow0 + r, col0 + 4 * q, w);
+                            }
+                        }
                     }
                 }
             }
@@ -511,6 +656,44 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
     }
 
     __syncthreads();
+    if (cta_split > 1) {
+        // The cluster's CTAs add their shares of the tile in order of K, each for its part of the
+        // outputs, from one another's shared memory.
+        cluster_sync_all();
+        if (unit < tiles) {
+            const Tile tl = tile_at(unit);
+            const int rows = min(128, tl.row_end - tl.row0);
+            const int quads = (glu ? BN / 2 : BN) / 4;
+            for (int i = (int)rank * C::THREADS + threadIdx.x; i < rows * quads; i += cta * C::THREADS) {
+                const int r = i / quads, q = i - r * quads;
+                const int64_t col = (int64_t)tl.ocol + 4 * q;
+                if (col >= a.ycols) continue;
+                auto sum = [&](int quad, float (&v)[4]) {
+                    const float4 *src = reinterpret_cast<const float4 *>(smem) + r * (BN / 4) + (quad ^ (r & 7));
+                    v[0] = v[1] = v[2] = v[3] = 0.0f;
+                    for (int p = 0; p < cta; ++p) {
+                        const float4 f = ld_shared_cluster_f4(mapa_shared(src, p));
+                        v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+                    }
+                };
+                float v[4];
+                sum(q, v);
+                if (glu) {
+                    float u[4];
+                    sum(BN / 8 + q, u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] *= silu_fast(u[j]);
+                } else {
+                    float b[4];
+                    bias_quad(a, tl.e, col, b);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] += b[j];
+                }
+                store_quad(a, (int64_t)tl.row0 + r, col, v);
+            }
+        }
+        cluster_sync_all();
+    }
     if constexpr (PAIR) cluster_sync_all();
     if (warp == 1) {
         __syncwarp();
@@ -523,13 +706,27 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN, PAIR>::THREADS), 1)
     if constexpr (PAIR) cluster_sync_all();
 }
 
-template <int KIND, int BN, bool PAIR>
-Status launch_blk(const LinearBlocksCall &c, cudaStream_t stream) {
-    using C = BlkCfg<KIND, BN, PAIR>;
+// split: CTAs that share a tile's K (one tile per cluster; the grid covers every tile).
+template <int KIND, int BN>
+Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
+    using C = BlkCfg<KIND, BN>;
+    constexpr bool PAIR = C::PAIR;
     constexpr int BK = C::F8 ? 128 : 64;
     alignas(64) CUtensorMap ta, tb;
-    TSFM_TRY(make_tmap_3d(&ta, c.x, KIND, c.K, c.M, 0, c.ldx, 0, BK, C::A_BOX));
-    TSFM_TRY(make_tmap_3d(&tb, c.w, KIND, c.K, c.N, c.groups, c.ldw, c.groups > 1 ? c.w_group : c.N * c.ldw, BK, BN / 2));
+    const bool glu = c.act == ACT_GLU;
+    {
+        const int64_t d[2] = {c.K, c.M}, st[2] = {1, c.ldx};
+        const uint32_t box[2] = {BK, C::A_BOX};
+        TSFM_TRY(make_tmap_nd(&ta, c.x, KIND, 2, d, st, box));
+    }
+    {
+        // W [groups, N, K]; for gated pairs [groups, N / 256, 2, 128, K].
+        const int64_t wg = c.groups > 1 ? c.w_group : c.N * c.ldw;
+        const int64_t d[5] = {c.K, glu ? 128 : c.N, glu ? 2 : 1, glu ? c.N / 256 : 1, c.groups};
+        const int64_t st[5] = {1, c.ldw, glu ? 128 * c.ldw : c.N * c.ldw, glu ? 256 * c.ldw : c.N * c.ldw, wg};
+        const uint32_t box[5] = {BK, (uint32_t)(PAIR || glu ? BN / 2 : BN), !PAIR && glu ? 2u : 1u, 1, 1};
+        TSFM_TRY(make_tmap_nd(&tb, c.w, KIND, 5, d, st, box));
+    }
     BlkArgs a;
     a.M = c.M;
     a.N = c.N;
@@ -547,39 +744,47 @@ Status launch_blk(const LinearBlocksCall &c, cudaStream_t stream) {
     a.bias = c.bias;
     a.y = c.y;
     a.ldy = c.ldy;
-    a.ycols = c.act == ACT_GLU ? c.N / 2 : c.N;
+    a.ycols = glu ? c.N / 2 : c.N;
     a.y_dtype = c.y_dtype;
     a.accumulate = c.accumulate;
     a.act = c.act;
     const int ysz = c.y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
-    a.vec = (reinterpret_cast<uintptr_t>(c.y) & 15) == 0 && (c.ldy * ysz) % 16 == 0;
+    a.vec = reinterpret_cast<uintptr_t>(c.y) % (4 * ysz) == 0 && c.ldy % 4 == 0;
+    a.vec32 = reinterpret_cast<uintptr_t>(c.y) % 32 == 0 && (c.ldy * ysz) % 32 == 0;
+    a.split = split;
     a.err = c.err;
     const int smem = C::smem(c.groups);
-    const void *fn = reinterpret_cast<const void *>(&linear_blocks_kernel<KIND, BN, PAIR>);
+    const void *fn = reinterpret_cast<const void *>(&linear_blocks_kernel<KIND, BN>);
     TSFM_TRY(ensure_smem_attr(fn, smem));
     // At most this many row tiles: every group may end inside one.
     const int64_t row_tiles = c.offsets ? c.M / C::TILE_M + std::min(c.groups, c.M) : (c.M + C::TILE_M - 1) / C::TILE_M;
     const int64_t most = row_tiles * a.n_tiles;
+    if (most > INT32_MAX / 16) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: too many tiles");
+    const int cta = PAIR ? 2 : split;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(PAIR ? 2 * std::min<int64_t>(most, num_sms() / 2) : std::min<int64_t>(most, num_sms())));
+    cfg.gridDim = dim3((unsigned)(split > 1 ? most * split : cta * std::min<int64_t>(most, num_sms() / cta)));
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = cta;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_blocks_kernel<KIND, BN, PAIR>, ta, tb, a);
+    cfg.numAttrs = cta > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_blocks_kernel<KIND, BN>, ta, tb, a);
     if (e != cudaSuccess) return Status::cuda(e, "linear (blocks): launch");
     return Status::ok();
 }
 
 template <int KIND>
 Status launch_kind(const LinearBlocksCall &c, cudaStream_t stream) {
-    return launch_blk<KIND, 128, false>(c, stream);
+    // Wide tiles once they fill the card: 256 x 256 on pairs of SMs, where the tensor cores are the
+    // bound; 128 x 128 below, which a group of a few rows wastes less of.
+    const int64_t rows = c.offsets ? c.M / c.groups : c.M;
+    if (rows > 128 && c.N > 128 && (c.M / 256) * ((c.N + 255) / 256) >= num_sms() / 2) return launch_blk<KIND, 256>(c, 1, stream);
+    return launch_blk<KIND, 128>(c, 1, stream);
 }
 
 }  // namespace
