@@ -15,6 +15,7 @@
 //               a tile holds g and u of the same columns.
 //   warp 1      tensor-memory allocation, MMA issue (one lane) into accumulators in tensor memory:
 //               one per tile (16 bits, two in turn) or one per block of K (E4M3).
+//   warp 2      E4M3, 256 columns: issues the TMA stores of the boxes that the epilogue fills.
 //   warp 3      E4M3: the scales of the tile's rows and columns into a ring of shared memory, four
 //               blocks of K at a time, ahead of the tiles that need them.
 //   warps 4..   epilogue: a thread owns a row and 128 (below 256 columns: 64) of its columns. The
@@ -48,7 +49,7 @@ constexpr int kMaxGroups = 1024;  // two words of shared memory each
 
 // Blocks of K whose scales share a slot of the ring, and the slots.
 constexpr int kScaleQuad = 4, kScaleSlots = 4;
-constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2) * 4;  // [block of K][row], then [half tile][block of K]
+constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2) * 4;  // [row][block of K], then [half tile][block of K]
 
 // KIND: element type of x and W (E_F16, E_BF16, E_U8 = E4M3).
 template <int KIND, int BN>
@@ -59,22 +60,25 @@ struct BlkCfg {
     static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
     static constexpr int TILE_M = PAIR ? 256 : 128;
-    static constexpr int A_BOX = BN == 256 ? 128 : 32;  // rows of x per TMA box
+    static constexpr int A_BOX = PAIR ? 128 : 32;  // rows of x per TMA box
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // rows of W in this CTA's shared memory
     static constexpr int B_BYTES = B_ROWS * 128;
-    static constexpr int STAGES = BN == 64 ? 8 : 5;
-    static constexpr int PRODUCERS = BN == 256 ? 1 : 2;
+    static constexpr int STAGES = BN == 64 ? 8 : PAIR && F8 ? 4 : 5;
+    static constexpr int PRODUCERS = PAIR ? 1 : 2;
     // Accumulators: NH column parts of BN / NH columns, NBUF of each.
     static constexpr int NH = F8 && BN == 256 ? 2 : 1;
     static constexpr int NBUF = !F8 || BN == 256 ? 2 : 512 / BN;
     static constexpr int TMEM_COLS = NBUF * BN;
+    // E4M3 on 256 columns stores 16-bit outputs by TMA from two 4 KB boxes per epilogue warp.
+    static constexpr bool TMA_Y = F8 && PAIR;
+    static constexpr int BOXES = TMA_Y ? 2 : 1;
     static constexpr int EPI_OFF = STAGES * (A_BYTES + B_BYTES);
-    static constexpr int SCALE_OFF = EPI_OFF + EPI_WARPS * 4096;
+    static constexpr int SCALE_OFF = EPI_OFF + EPI_WARPS * BOXES * 4096;
     static constexpr int BAR_OFF = SCALE_OFF + (F8 ? kScaleSlots * kScaleSlotBytes : 0);
     static constexpr int GROUP_OFF = BAR_OFF + 512;
     static int smem(int64_t groups) { return 1024 + GROUP_OFF + 8 * (int)(groups + 1); }
-    static_assert((2 * STAGES + 2 * NH * NBUF + 2 * kScaleSlots + 2) * 8 <= 512, "barriers");
+    static_assert((2 * STAGES + 2 * NH * NBUF + 2 * kScaleSlots + 2 * EPI_WARPS + 2) * 8 <= 512, "barriers");
 };
 
 struct BlkArgs {
@@ -90,9 +94,15 @@ struct BlkArgs {
     int y_dtype, accumulate, act;
     int vec;       // y's base and row stride suit 4-element stores
     int vec32;     // and 32-byte ones
+    int y_tma;     // tiles leave through tmY
     int split;     // CTAs of a cluster that share a tile's K (1: none)
     int *err;
 };
+
+__device__ __forceinline__ uint4 pack8(bool f16, const float *v) {
+    if (f16) return make_uint4(pack16<true>(v[0], v[1]), pack16<true>(v[2], v[3]), pack16<true>(v[4], v[5]), pack16<true>(v[6], v[7]));
+    return make_uint4(pack16<false>(v[0], v[1]), pack16<false>(v[2], v[3]), pack16<false>(v[4], v[5]), pack16<false>(v[6], v[7]));
+}
 
 __device__ __forceinline__ float silu_fast(float u) { return __fdividef(u, 1.0f + __expf(-u)); }
 
@@ -163,16 +173,16 @@ __device__ __forceinline__ void store_sectors(void *o, const float (&v)[32]) {
 template <int KIND, int BN>
 __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     linear_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                         BlkArgs a) {
+                         const __grid_constant__ CUtensorMap tmY, BlkArgs a) {
     using C = BlkCfg<KIND, BN>;
     constexpr bool F8 = C::F8, PAIR = C::PAIR;
     constexpr int STAGES = C::STAGES, NBUF = C::NBUF, NH = C::NH;
     constexpr int BK = F8 ? 128 : 64;  // elements of K per stage
     // 384 threads launch with 168 registers each; the epilogue's two warpgroups (128 sums and 64 loaded
-    // values a thread) take them from the first one: 64,512 = 128 x 56 + 256 x 224.
+    // values a thread) take them from the first one: 64,512 = 128 x 40 + 256 x 232.
     constexpr bool SPLIT_REGS = F8 && BN == 256;
     constexpr uint32_t IDESC = idesc_f32acc(KIND == E_BF16 ? 1u : 0u, C::TILE_M, BN / NH);
-    const int cta_split = BN == 256 ? 1 : a.split;  // CTAs that share a tile's K
+    const int cta_split = PAIR ? 1 : a.split;  // CTAs that share a tile's K
     const int cta = PAIR ? 2 : cta_split;           // CTAs of a cluster
     const uint32_t rank = cta > 1 ? cluster_ctarank() : 0u;
     const bool leader = !PAIR || rank == 0;
@@ -188,7 +198,9 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     uint64_t *pempty = pfull + NH * NBUF;
     uint64_t *sfull = pempty + NH * NBUF;   // scales
     uint64_t *sempty = sfull + kScaleSlots;
-    uint64_t *drain = sempty + kScaleSlots;
+    uint64_t *bfull = sempty + kScaleSlots;  // staging boxes, per epilogue warp
+    uint64_t *bempty = bfull + C::EPI_WARPS;
+    uint64_t *drain = bempty + C::EPI_WARPS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *g_row = reinterpret_cast<int *>(smem + C::GROUP_OFF);  // group e has rows [g_row[e], g_row[e + 1])
@@ -205,6 +217,10 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
             mbar_init(&pfull[i], 1);
             mbar_init(&pempty[i], (PAIR ? 2 : 1) * C::EPI_WARPS / NH);  // one arrival per epilogue warp
         }
+        for (int i = 0; i < C::EPI_WARPS; ++i) {
+            mbar_init(&bfull[i], 1);
+            mbar_init(&bempty[i], 1);
+        }
         for (int i = 0; i < kScaleSlots; ++i) {
             mbar_init(&sfull[i], 32);
             mbar_init(&sempty[i], C::EPI_WARPS);
@@ -215,9 +231,17 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
     }
-    if (warp == 0) {
+    if (warp == 0 && a.offsets == nullptr) {
+        if (lane == 0) {
+            g_row[0] = g_tile[0] = 0;
+            g_row[1] = (int)a.M;
+            g_tile[1] = (int)((a.M + C::TILE_M - 1) / C::TILE_M);
+        }
+    } else if (warp == 0) {
         const int M = (int)a.M;
-        int end = a.offsets ? min(max(a.offsets[0], 0), M) : 0;  // running maximum of the offsets
+        const int first = __ldg(a.offsets);
+        int o = lane < a.groups ? __ldg(a.offsets + lane + 1) : 0;
+        int end = min(max(first, 0), M);  // running maximum of the offsets
         int tiles = 0;
         if (lane == 0) {
             g_row[0] = end;
@@ -225,8 +249,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
         }
         for (int base = 0; base < a.groups; base += 32) {
             const int e = base + lane;
-            int o = e < a.groups ? (a.offsets ? min(max(a.offsets[e + 1], 0), M) : M) : 0;
-            o = max(o, end);
+            o = max(min(max(o, 0), M), end);
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const int p = __shfl_up_sync(0xffffffffu, o, d);
@@ -246,6 +269,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
             }
             end = __shfl_sync(0xffffffffu, o, 31);
             tiles += __shfl_sync(0xffffffffu, t, 31);
+            o = e + 32 < a.groups ? __ldg(a.offsets + e + 33) : 0;
         }
     }
     if (warp == 1) {
@@ -308,7 +332,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     };
 
     if (warp < 4) {
-        if constexpr (SPLIT_REGS) regs_dec<56>();
+        if constexpr (SPLIT_REGS) regs_dec<40>();
         if (warp == 0 || (C::PRODUCERS == 2 && warp == 2)) {
             // Producers: of two, stage use number i (over all tiles) belongs to warp 2 (i % 2).
             const bool el = elect_one();
@@ -331,7 +355,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                             if (leader) mbar_arrive_expect_tx(&full[s], 2 * (C::A_BYTES + C::B_BYTES));
                             const uint32_t fb = mapa_shared(&full[s], 0);
                             tma_load_2d_pair(sA + s * C::A_BYTES, &tmA, fb, kc, tl.row0);
-                            tma_load_5d_pair(sB + s * C::B_BYTES, &tmB, fb, kc, glu ? 0 : c1 + (int)rank * (BN / 2),
+                            tma_load_5d_pair(sB + s * C::B_BYTES, &tmB, fb, kc, glu ? c1 : c1 + (int)rank * (BN / 2),
                                              glu ? (int)rank : 0, c3, tl.e);
                         } else {
                             mbar_arrive_expect_tx(&full[s], na * C::A_BOX * 128 + C::B_BYTES);
@@ -445,8 +469,39 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                 }
                 __syncwarp();
             }
+        } else if (C::TMA_Y && warp == 2) {
+            // Stores: the boxes of every epilogue warp, a tile at a time (a warp whose rows end inside its
+            // 32 has stored them itself).
+            if (a.y_tma) {
+                const bool el = elect_one();
+                uint32_t bph = 0;
+                bool ok = true;
+                for (int t = unit; t < tiles && ok; t += units, bph ^= 1u) {
+                    const Tile tl = tile_at(t);
+                    for (int w = 0; w < C::EPI_WARPS; ++w) {
+                        ok = wait(&bfull[w], bph, ERR_SITE_BLOCKS_EPILOGUE);
+                        if (!ok) break;
+                        const int wrow0 = tl.row0 + (w & 3) * 32, wrows = tl.row_end - wrow0;
+                        if (el && (wrows >= 32 || (wrows > 0 && a.offsets == nullptr))) {
+                            const uint8_t *b = smem + C::EPI_OFF + w * C::BOXES * 4096;
+                            const int col0 = tl.ocol + (w >> 2) * 64, col1 = tl.b1 + (w >> 2) * 64;
+                            if (col0 < a.ycols) tma_store_2d(&tmY, b, col0, wrow0);
+                            if (!glu && col1 < a.ycols) tma_store_2d(&tmY, b + 4096, col1, wrow0);
+                            bulk_commit();
+                        }
+                    }
+                    if (el) {
+                        bulk_wait_read_0();
+                        for (int w = 0; w < C::EPI_WARPS; ++w) mbar_arrive(&bempty[w]);
+                    }
+                    __syncwarp();
+                }
+                // Every box has been written before the CTA exits.
+                if (el) bulk_wait_all();
+                __syncwarp();
+            }
         } else if (F8 && warp == 3) {
-            // Scales: slot = xs[4][128] then ws[2][4] (the half tiles' column blocks), by asynchronous
+            // Scales: slot = xs[128][4] then ws[2][4] (the half tiles' column blocks), by asynchronous
             // copies; entries past this CTA's last block of K are not read.
             int slot = 0;
             uint32_t ph = 0;
@@ -464,7 +519,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     const int n = min(kScaleQuad, kb1 - kb);
                     for (int r = lane; r < 128; r += 32) {
                         const float *src = xs + (int64_t)min(r, last) * a.ld_xs + kb;
-                        for (int j = 0; j < n; ++j) cp_async_4(d + j * 512 + r * 4, src + j);
+                        for (int j = 0; j < n; ++j) cp_async_4(d + r * 16 + j * 4, src + j);
                     }
                     if (lane < 8 && (lane & 3) < n) cp_async_4(d + 2048 + lane * 4, ws + kb);
                     cp_async_arrive(&sfull[slot]);
@@ -477,16 +532,16 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
             cp_async_wait_all();
         }
     } else {
-        if constexpr (SPLIT_REGS) regs_inc<224>();
+        if constexpr (SPLIT_REGS) regs_inc<232>();
         constexpr int PARTS = C::EPI_WARPS / 4;  // warps that share a row's columns
         constexpr int CH = BN / PARTS / 32;      // 32-column chunks per thread
         constexpr int CPH = CH / 2;              // of each half of the tile
         const int ew = warp - 4;
         const int eg = warp & 3, part = ew >> 2;  // tensor-memory lanes [32 eg, 32 eg + 32)
         const int half = NH == 2 ? part : 0;      // this warp's accumulators
-        float4 *box = reinterpret_cast<float4 *>(smem + C::EPI_OFF + ew * 4096);
+        float4 *box = reinterpret_cast<float4 *>(smem + C::EPI_OFF + ew * C::BOXES * 4096);
         int buf = 0, slot = 0;
-        uint32_t bph = 0, sph = 0;
+        uint32_t bph = 0, sph = 0, boxph = 0;
         bool ok = true;
         auto wait_epi = [&](uint64_t *bar, uint32_t parity) { return wait(bar, parity, ERR_SITE_BLOCKS_EPILOGUE); };
         const uint32_t handback = PAIR ? mapa_shared(&pempty[half * NBUF], 0) : 0u;  // the MMA-issuing CTA's barriers
@@ -508,28 +563,12 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
         // Gated pairs: chunk c < CPH is g's, chunk c + CPH the same columns of u.
         auto acol = [&](int c) { return NH == 2 ? c * 32 : (c / CPH) * (BN / 2) + (part * CPH + c % CPH) * 32; };
         auto ycol = [&](const Tile &tl, int c) { return (c < CPH ? tl.ocol : tl.b1) + (part * CPH + c % CPH) * 32; };
-        // The scales of the next block of K (over all tiles): the row's times each half's.
-        float s0 = 0.0f, s1 = 0.0f;
         const uint32_t scales = smem_u32(smem) + C::SCALE_OFF;
-        auto next_scales = [&](int kb) {
-            const int j = kb & (kScaleQuad - 1);
-            // (A wait that gave up has raised the abort flag: the next accumulator's ends the loops.)
-            if (j == 0) wait_epi(&sfull[slot], sph);
-            const uint32_t sc = scales + slot * kScaleSlotBytes;
-            const float sx = ld_shared_f32(sc + j * 512 + (eg * 32 + lane) * 4);
-            s0 = sx * ld_shared_f32(sc + 2048 + j * 4);
-            s1 = sx * ld_shared_f32(sc + 2048 + 16 + j * 4);
-            if (j == kScaleQuad - 1 || kb == kbn - 1) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sempty[slot]);
-                if (++slot == kScaleSlots) {
-                    slot = 0;
-                    sph ^= 1u;
-                }
-            }
-        };
-        if (F8 && unit < tiles) next_scales(0);
         for (int t = unit; t < tiles && ok; t += units) {
+            if (a.bias && lane < CH && !glu) {  // on its way while the sums are made
+                const Tile tl = tile_at(t);
+                prefetch_l1(a.bias + tl.e * a.N + min((int64_t)ycol(tl, lane), a.N - 1));
+            }
             float2 acc[F8 ? CH : 1][16];
             uint32_t tbase = 0;
             if constexpr (F8) {
@@ -537,28 +576,53 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) acc[c][j] = make_float2(0.0f, 0.0f);
-                for (int kb = 0; kb < kbn; ++kb) {
-                    ok = wait_epi(&pfull[half * NBUF + buf], bph);
+                for (int kb = 0; kb < kbn && ok; kb += kScaleQuad) {
+                    // Four blocks' scales at once (a read per block, behind the accumulator's loads in the
+                    // same queue, cost 150 cycles each): the row's times each half's.
+                    ok = wait_epi(&sfull[slot], sph);
                     if (!ok) break;
-                    tc_fence_after();
-                    tbase = tmem_base + ((uint32_t)(eg * 32) << 16) + (uint32_t)((half * NBUF + buf) * (BN / NH));
-                    // The accumulator is handed back, and the next scales are read, before the last additions.
+                    const uint32_t sc = scales + slot * kScaleSlotBytes;
+                    float xv[4], w0[4], w1[4], s0[4], s1[4];
+                    ld_shared_v4(sc + (eg * 32 + lane) * 16, xv);
+                    ld_shared_v4(sc + 2048, w0);
+                    ld_shared_v4(sc + 2064, w1);
 #pragma unroll
-                    for (int c = 0; c < CH; c += 2) {
-                        float p[2][32];
-                        tmem_ld32f(tbase + acol(c), p[0]);
-                        tmem_ld32f(tbase + acol(c + 1), p[1]);
-                        tmem_wait_ld();
-                        const float2 sa = c < CPH ? make_float2(s0, s0) : make_float2(s1, s1);
-                        const float2 sb = c + 1 < CPH ? make_float2(s0, s0) : make_float2(s1, s1);
-                        if (c + 2 == CH) {
-                            release();
-                            if (kb + 1 < kbn || t + units < tiles) next_scales(kb + 1 < kbn ? kb + 1 : 0);
+                    for (int j = 0; j < kScaleQuad; ++j) s0[j] = xv[j] * w0[j], s1[j] = xv[j] * w1[j];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[slot]);
+                    if (++slot == kScaleSlots) {
+                        slot = 0;
+                        sph ^= 1u;
+                    }
+                    const int n = min(kScaleQuad, kbn - kb);
+#pragma unroll 1
+                    for (int j = 0; j < n; ++j) {
+                        ok = wait_epi(&pfull[half * NBUF + buf], bph);
+                        if (!ok) break;
+                        tc_fence_after();
+                        tbase = tmem_base + ((uint32_t)(eg * 32) << 16) + (uint32_t)((half * NBUF + buf) * (BN / NH));
+                        // A chunk loads while the one before it is added; the accumulator is handed back before
+                        // the last additions.
+                        float p0[32], p1[32];
+                        tmem_ld32f(tbase + acol(0), p0);
+#pragma unroll
+                        for (int c = 0; c < CH; c += 2) {
+                            tmem_wait_ld();
+                            tmem_ld32f(tbase + acol(c + 1), p1);
+                            const float2 sa = c < CPH ? make_float2(s0[0], s0[0]) : make_float2(s1[0], s1[0]);
+                            const float2 sb = c + 1 < CPH ? make_float2(s0[0], s0[0]) : make_float2(s1[0], s1[0]);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) fma_f32x2(acc[c][i], make_float2(p0[2 * i], p0[2 * i + 1]), sa);
+                            tmem_wait_ld();
+                            if (c + 2 < CH)
+                                tmem_ld32f(tbase + acol(c + 2), p0);
+                            else
+                                release();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) fma_f32x2(acc[c + 1][i], make_float2(p1[2 * i], p1[2 * i + 1]), sb);
                         }
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c][j], make_float2(p[0][2 * j], p[0][2 * j + 1]), sa);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c + 1][j], make_float2(p[1][2 * j], p[1][2 * j + 1]), sb);
+                        for (int q = 0; q < kScaleQuad - 1; ++q) s0[q] = s0[q + 1], s1[q] = s1[q + 1];
                     }
                 }
                 if (!ok) break;
@@ -596,7 +660,15 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     chunk(c, v);
                     dump(v, to + acol(c) / 4);
                 }
-            } else if (wrows > 0) {
+            }
+            const bool tma = C::TMA_Y && a.y_tma;
+            const bool boxed = tma && (wrows == 32 || (wrows > 0 && a.offsets == nullptr));
+            if (tma) {
+                ok = wait_epi(&bempty[ew], boxph ^ 1u);
+                if (!ok) break;
+                boxph ^= 1u;
+            }
+            if (wrows > 0 && cta_split == 1) {
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     if (glu && c >= CPH) break;
@@ -609,17 +681,24 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] *= silu_fast(u[j]);
                     } else if (a.bias) {
-                        const float *b = a.bias + tl.e * a.N + col0;
-                        if (col0 + 32 <= a.N) {
+                        // (columns past N, which are not stored, repeat the last one's)
+                        const float *b = a.bias + tl.e * a.N;
+                        const int last = (int)a.N - 1;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] += __ldg(b + j);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (col0 + j < a.N) v[j] += __ldg(b + j);
-                        }
+                        for (int j = 0; j < 32; ++j) v[j] += __ldg(b + min(col0 + j, last));
                     }
-                    if (a.vec32 && col0 + 32 <= a.ycols && !a.accumulate) {
+                    if (boxed) {
+                        // 64-column boxes (rows past M and columns past N are clipped): the tile leaves while
+                        // the next one is summed.
+                        if (a.act == 1) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = fmaxf(v[j], 0.0f);
+                        }
+                        const bool f16 = a.y_dtype == TSFM_DTYPE_F16;
+                        uint4 *b = reinterpret_cast<uint4 *>(box) + (c / 2) * 256 + lane * 8;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) b[(4 * (c & 1) + q) ^ (lane & 7)] = pack8(f16, v + 8 * q);
+                    } else if (a.vec32 && col0 + 32 <= a.ycols && !a.accumulate) {
                         // A thread's 32 columns are whole 32-byte sectors of its row.
                         if (a.act == 1) {
 #pragma unroll
@@ -650,6 +729,11 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                         }
                     }
                 }
+            }
+            if (tma) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bfull[ew]);
             }
             if constexpr (!F8) release();
         }
@@ -712,7 +796,7 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     using C = BlkCfg<KIND, BN>;
     constexpr bool PAIR = C::PAIR;
     constexpr int BK = C::F8 ? 128 : 64;
-    alignas(64) CUtensorMap ta, tb;
+    alignas(64) CUtensorMap ta, tb, ty;
     const bool glu = c.act == ACT_GLU;
     {
         const int64_t d[2] = {c.K, c.M}, st[2] = {1, c.ldx};
@@ -751,6 +835,13 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     const int ysz = c.y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
     a.vec = reinterpret_cast<uintptr_t>(c.y) % (4 * ysz) == 0 && c.ldy % 4 == 0;
     a.vec32 = reinterpret_cast<uintptr_t>(c.y) % 32 == 0 && (c.ldy * ysz) % 32 == 0;
+    a.y_tma = C::TMA_Y && ysz == 2 && !c.accumulate && reinterpret_cast<uintptr_t>(c.y) % 16 == 0 && c.ldy % 8 == 0;
+    ty = ta;
+    if (a.y_tma) {
+        const int64_t d[2] = {a.ycols, c.M}, st[2] = {1, c.ldy};
+        const uint32_t box[2] = {64, 32};
+        TSFM_TRY(make_tmap_nd(&ty, c.y, c.y_dtype == TSFM_DTYPE_F16 ? E_F16 : E_BF16, 2, d, st, box));
+    }
     a.split = split;
     a.err = c.err;
     const int smem = C::smem(c.groups);
@@ -773,7 +864,7 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cta > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_blocks_kernel<KIND, BN>, ta, tb, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_blocks_kernel<KIND, BN>, ta, tb, ty, a);
     if (e != cudaSuccess) return Status::cuda(e, "linear (blocks): launch");
     return Status::ok();
 }

@@ -14,6 +14,7 @@
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace tsfm {
 
@@ -35,31 +36,47 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits) {
     return {__uint_as_float((uint32_t)e << 23), __uint_as_float((uint32_t)(254 - e) << 23)};
 }
 
-// Eight consecutive elements of a row as FP32; elements at or past `n` read as zero.
+// Eight consecutive elements of a row as they are stored; elements at or past `n` read as zero.
 template <int DT>
-__device__ __forceinline__ void load8(const void *row, int64_t col, int n, bool vec, float (&v)[8]) {
-    if constexpr (DT == E_F32X) {
-        const float *p = static_cast<const float *>(row) + col;
-        if (vec && n >= 8) {
-            const float4 a = __ldcs(reinterpret_cast<const float4 *>(p));
-            const float4 b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
+struct Raw8 {
+    uint4 w[DT == E_F32X ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const void *row, int64_t col, int n, bool vec) {
+    Raw8<DT> r;
+    constexpr int W = DT == E_F32X ? 2 : 1;
+    if (vec && n >= 8) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + col * (DT == E_F32X ? 4 : 2));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.0f;
+        for (int i = 0; i < W; ++i) r.w[i] = __ldcs(p + i);
+    } else {
+        uint32_t w[4 * W];
+#pragma unroll
+        for (int j = 0; j < 4 * W; ++j) {
+            if constexpr (DT == E_F32X) {
+                w[j] = j < n ? static_cast<const uint32_t *>(row)[col + j] : 0u;
+            } else {
+                const uint16_t *p = static_cast<const uint16_t *>(row) + col;
+                w[j] = (2 * j < n ? (uint32_t)p[2 * j] : 0u) | (2 * j + 1 < n ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+    return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void to_f32(const Raw8<DT> &r, float (&v)[8]) {
+    if constexpr (DT == E_F32X) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v[4 * i] = __uint_as_float(r.w[i].x), v[4 * i + 1] = __uint_as_float(r.w[i].y);
+            v[4 * i + 2] = __uint_as_float(r.w[i].z), v[4 * i + 3] = __uint_as_float(r.w[i].w);
         }
     } else {
-        const uint16_t *p = static_cast<const uint16_t *>(row) + col;
-        uint32_t w[4];
-        if (vec && n >= 8) {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(p));
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[j] = (2 * j < n ? (uint32_t)p[2 * j] : 0u) | (2 * j + 1 < n ? (uint32_t)p[2 * j + 1] << 16 : 0u);
-        }
+        const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (DT == E_F16) {
@@ -94,26 +111,41 @@ __device__ __forceinline__ void store8(uint8_t *p, int n, bool vec, const float 
     }
 }
 
-// One row x 128 columns per half warp: 16 lanes of 8 elements.
-template <int DT>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeCall c, int64_t blocks, int64_t per_row, bool vx,
+// One row x 128 columns per half warp: 16 lanes of 8 elements. A half warp takes U blocks, all of
+// whose loads are under way before the first maximum; the CTA's 16 U blocks are consecutive.
+template <int DT, int U>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeCall c, int64_t blocks, uint32_t per_row, bool vx,
                                                             bool vq) {
+    constexpr int esz = DT == E_F32X ? 4 : 2;
     const int lane = threadIdx.x & 15;
-    const int64_t step = (int64_t)gridDim.x * (blockDim.x / 16);
-    for (int64_t b = (int64_t)blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 4); b < blocks; b += step) {
-        const int64_t r = b / per_row, kb = b - r * per_row;
-        const int64_t col = kb * 128 + lane * 8;
-        const int n = (int)max((int64_t)0, min((int64_t)8, c.cols - col));
-        constexpr int esz = DT == E_F32X ? 4 : 2;
-        float v[8];
-        load8<DT>(static_cast<const char *>(c.x) + r * c.ldx * esz, col, n, vx, v);
-        uint32_t m = amax8(v);
-        const uint32_t half = 0xffffu << (threadIdx.x & 16);
+    const int64_t first = (int64_t)blockIdx.x * (16 * U);
+    const int64_t r0 = first / per_row;
+    const uint32_t kb0 = (uint32_t)(first - r0 * per_row);
+    Raw8<DT> raw[U];
+    int64_t row[U];
+    uint32_t kb[U];
+    int n[U];
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half, m, o));
+    for (int u = 0; u < U; ++u) {
+        const uint32_t b = u * 16 + (threadIdx.x >> 4), k = kb0 + b, q = k / per_row;
+        row[u] = r0 + q;
+        kb[u] = k - q * per_row;
+        const int64_t col = (int64_t)kb[u] * 128 + lane * 8;
+        n[u] = first + b < blocks ? (int)max((int64_t)0, min((int64_t)8, c.cols - col)) : 0;
+        raw[u] = load8<DT>(static_cast<const char *>(c.x) + (n[u] > 0 ? row[u] : 0) * c.ldx * esz, col, n[u], vx);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float v[8];
+        to_f32<DT>(raw[u], v);
+        uint32_t m = amax8(v);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         const BlockScale s = block_scale(m);
-        if (lane == 0) c.scale[r * c.ld_scale + kb] = s.scale;
-        store8(c.q + r * c.ldq + col, n, vq, v, s.inv);
+        if (n[u] > 0) {
+            if (lane == 0) c.scale[row[u] * c.ld_scale + kb[u]] = s.scale;
+            store8(c.q + row[u] * c.ldq + kb[u] * 128 + lane * 8, n[u], vq, v, s.inv);
+        }
     }
 }
 
@@ -127,15 +159,19 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(QuantizeCall c, boo
     const int n = (int)max((int64_t)0, min((int64_t)8, c.cols - col));
     constexpr int esz = DT == E_F32X ? 4 : 2;
     for (int64_t br = blockIdx.y; br * 128 < c.rows; br += gridDim.y) {
-        float v[8][8];
+        Raw8<DT> raw[8];
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t r = br * 128 + i * 16 + r0;
-            load8<DT>(static_cast<const char *>(c.x) + r * c.ldx * esz, col, r < c.rows ? n : 0, vx, v[i]);
+            raw[i] = load8<DT>(static_cast<const char *>(c.x) + r * c.ldx * esz, col, r < c.rows ? n : 0, vx);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, amax8(v[i]));
+        for (int i = 0; i < 8; ++i) {
+            float v[8];
+            to_f32<DT>(raw[i], v);
+            m = max(m, amax8(v));
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
@@ -148,7 +184,9 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(QuantizeCall c, boo
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t r = br * 128 + i * 16 + r0;
-            if (r < c.rows) store8(c.q + r * c.ldq + col, n, vq, v[i], s.inv);
+            float v[8];
+            to_f32<DT>(raw[i], v);
+            if (r < c.rows) store8(c.q + r * c.ldq + col, n, vq, v, s.inv);
         }
     }
 }
@@ -161,9 +199,10 @@ Status launch_dt(const QuantizeCall &c, cudaStream_t stream) {
     const int64_t per_row = (c.cols + 127) / 128;
     if (c.block_rows == 1) {
         const int64_t blocks = c.rows * per_row;
-        const int64_t ctas = (blocks + 15) / 16;
-        const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)num_sms() * 8);
-        quantize_rows_kernel<DT><<<grid, 256, 0, stream>>>(c, blocks, per_row, vx, vq);
+        constexpr int U = DT == E_F32X ? 2 : 4;  // 64 bytes a thread in flight
+        const int64_t ctas = (blocks + 16 * U - 1) / (16 * U);
+        if (ctas > INT32_MAX) return Status::fail(TSFM_ERR_UNSUPPORTED, "quantize: too many blocks");
+        quantize_rows_kernel<DT, U><<<(unsigned)ctas, 256, 0, stream>>>(c, blocks, (uint32_t)per_row, vx, vq);
     } else {
         const int64_t tiles = (c.rows + 127) / 128;
         const dim3 grid((unsigned)per_row, (unsigned)std::min<int64_t>(tiles, 65535));
