@@ -224,6 +224,71 @@ def test_linear_e4m3(M, N, K):
     c.check(torch.float16, pad=8)
 
 
+# Tile widths by the size of the product: 64 columns with K shared by 2 to 8 CTAs of a cluster (long K,
+# few tiles; rows and columns that end inside a tile, a K that its CTAs share unevenly), 128 columns,
+# and 256 x 256 on pairs of SMs, with full and ragged edges.
+WIDTHS = [(1, 1024, 4096), (3, 500, 8200), (130, 1000, 2050), (200, 70, 2176), (256, 512, 6000), (2048, 768, 768),
+          (2100, 1030, 520), (6000, 2500, 2100), (4096, 4096, 1024), (9000, 2304, 392)]
+
+
+@pytest.mark.parametrize("M,N,K", WIDTHS)
+def test_linear_e4m3_tile_widths(M, N, K):
+    c = Case(M, N, K, "e4m3", bias=True, seed=3)
+    c.check(torch.float32)
+    c.check(torch.float16, act=1)
+    c.check(torch.bfloat16, pad=8)    # rows of 16-byte multiples
+    c.check(torch.bfloat16, pad=3, shift=1)
+    c.check(accumulate=1, act=1)
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 512, 4096), (300, 512, 2048), (8000, 2048, 1024)])
+def test_linear_e4m3_gated_tile_widths(M, N, K):
+    c = Case(M, N, K, "e4m3", seed=4)
+    k = 0.5 / float(c.ref.std())
+    c.xs *= k
+    c.ref, c.tol = c.ref * k, 1.1 * c.tol * k
+    c.check(torch.bfloat16, act=3)
+    c.check(torch.float16, act=3, pad=2)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", torch.bfloat16, torch.float16], ids=str)
+def test_grouped_wide_tiles(kind):
+    # groups of many rows on 256 x 256 tiles, some of few, some that end one row into a tile
+    counts = [3000, 0, 257, 2048, 1, 1500, 255, 4097]
+    c = Case(sum(counts) + 7, 1100, 1030, kind, counts=counts, first=5, bias=True)
+    c.check(torch.bfloat16, act=1)
+    c.check(torch.float32, pad=4)
+    c.check(torch.float16, pad=1, shift=1)
+    c.check(torch.float32, accumulate=1)
+    g = Case(sum(counts), 1024, 640, kind, counts=counts)
+    if kind == "e4m3":
+        k = 0.5 / float(g.ref.std())
+        g.xs *= k
+        g.ref, g.tol = g.ref * k, 1.1 * g.tol * k
+    g.check(torch.float16 if kind == "e4m3" else kind, act=3)
+
+
+def test_linear_e4m3_offsets_past_32_bits():
+    # y of more than 2^31 elements and x of more than 2^31 bytes: the last rows and columns
+    M, N, K = 140000, 16384, 16400
+    g = gen(9)
+    x = torch.zeros(M, K, device="cuda", dtype=torch.uint8)
+    w = torch.zeros(N, K, device="cuda", dtype=torch.uint8)
+    x[-3:] = 0x38  # 1.0
+    w[-2:] = 0x40  # 2.0
+    kb, nb = -(-K // 128), N // 128
+    xs, ws = torch.ones(M, kb, device="cuda"), torch.full((nb, kb), 0.5, device="cuda")
+    y = torch.full((M, N), 7.0, device="cuda", dtype=torch.bfloat16)
+    tb.check(tb.lib.tsfm_kernel_linear_e4m3(ptr(x), ptr(xs), kb, ptr(w), ptr(ws), kb, None, ptr(y), 2, 0, 0, M, N, K, K, K,
+                                            N, stream()))
+    torch.cuda.synchronize()
+    # 16400 ones times 2 times 0.5, rounded to bf16
+    assert (y[-3:, -2:] == torch.tensor(16400.0).bfloat16().item()).all()
+    assert (y[-3:, :-2] == 0).all() and (y[:-3] == 0).all()
+    del x, w, y, xs, ws, g
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 256, 100), (50, 512, 768), (300, 1024, 320), (2000, 2048, 1024)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_linear_e4m3_gated(M, N, K, dtype):

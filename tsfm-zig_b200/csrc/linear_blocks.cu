@@ -39,6 +39,7 @@
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace tsfm {
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     // values a thread) take them from the first one: 64,512 = 128 x 40 + 256 x 232.
     constexpr bool SPLIT_REGS = F8 && BN == 256;
     constexpr uint32_t IDESC = idesc_f32acc(KIND == E_BF16 ? 1u : 0u, C::TILE_M, BN / NH);
-    const int cta_split = PAIR ? 1 : a.split;  // CTAs that share a tile's K
+    const int cta_split = F8 && BN == 64 ? a.split : 1;  // CTAs that share a tile's K
     const int cta = PAIR ? 2 : cta_split;           // CTAs of a cluster
     const uint32_t rank = cta > 1 ? cluster_ctarank() : 0u;
     const bool leader = !PAIR || rank == 0;
@@ -790,7 +791,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     if constexpr (PAIR) cluster_sync_all();
 }
 
-// split: CTAs that share a tile's K (one tile per cluster; the grid covers every tile).
+// split: CTAs that share a tile's K (64-wide E4M3 tiles; one tile per cluster, the grid covers every tile).
 template <int KIND, int BN>
 Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     using C = BlkCfg<KIND, BN>;
@@ -869,13 +870,55 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     return Status::ok();
 }
 
+// The tile width by the time that its waves of tiles take: a start, and per wave a part per stage of
+// K and one per tile (units of 100 ns, fitted to M 1-4096, N 768-4096, K 768-4096; the fit need only
+// rank the widths). Groups: each is taken to end in the middle of a tile. Measured, E4M3, us for widths
+// 64 / 128 / 256:
+//   M 512  N 2304 K 768   6.6 /  7.0 / 10.8      M 2048 N 4096 K 1024  24.1 / 19.7 / 18.6
+//   M 1024 N 2304 K 768   8.9 /  7.3 / 11.2      M 4096 N 4096 K 1024  42.8 / 30.5 / 29.2
+//   M 2048 N 1024 K 4096 22.6 / 15.6 / 22.8      M 4096 N 1024 K 4096  40.4 / 27.4 / 24.3
+template <int KIND>
+int tile_width(const LinearBlocksCall &c) {
+    struct Cost {
+        int bn, rows, units;
+        double start, stage, tile;
+    };
+    const int sms = num_sms();
+    const bool f8 = KIND == E_U8;
+    const Cost costs[3] = {{64, 128, sms, 0, f8 ? 2.6 : 2.2, f8 ? 6.0 : 3.0},
+                           {128, 128, sms, 0, f8 ? 3.0 : 2.8, f8 ? 8.0 : 3.0},
+                           {256, 256, sms / 2, f8 ? 30.0 : 35.0, f8 ? 4.4 : 3.6, f8 ? 12.0 : 5.0}};
+    const int64_t stages = (c.K + (f8 ? 127 : 63)) / (f8 ? 128 : 64);
+    int best = 128;
+    double least = 1e300;
+    for (const Cost &k : costs) {
+        const int64_t ends = c.offsets ? std::min(c.groups, c.M) : 1;
+        const int64_t row_tiles = std::max(ends, c.M / k.rows + (c.offsets ? ends / 2 : c.M % k.rows != 0));
+        const double tiles = (double)row_tiles * (double)((c.N + k.bn - 1) / k.bn);
+        const double t = k.start + std::ceil(tiles / k.units) * (k.stage * (double)stages + k.tile);
+        if (t < least) {
+            least = t;
+            best = k.bn;
+        }
+    }
+    return best;
+}
+
 template <int KIND>
 Status launch_kind(const LinearBlocksCall &c, cudaStream_t stream) {
-    // Wide tiles once they fill the card: 256 x 256 on pairs of SMs, where the tensor cores are the
-    // bound; 128 x 128 below, which a group of a few rows wastes less of.
-    const int64_t rows = c.offsets ? c.M / c.groups : c.M;
-    if (rows > 128 && c.N > 128 && (c.M / 256) * ((c.N + 255) / 256) >= num_sms() / 2) return launch_blk<KIND, 256>(c, 1, stream);
-    return launch_blk<KIND, 128>(c, 1, stream);
+    const int bn = tile_width<KIND>(c);
+    if (bn == 256) return launch_blk<KIND, 256>(c, 1, stream);
+    if (bn == 128) return launch_blk<KIND, 128>(c, 1, stream);
+    // Few tiles and a long K (one group, 16 blocks of K or more): 2, 4 or 8 CTAs of a cluster share a
+    // tile's K, as many as leave all clusters on the card at once (of 8 CTAs, 16 clusters took two
+    // turns). us for 1 / 2 / 4 / 8 CTAs: M 32 N 1024 K 4096 12.6 / 9.7 / 7.7 / 12.9, M 32 N 512 K 8192
+    // 21.0 / 13.9 / 9.7 / 7.9. At K 768 the exchange costs more than it saves (N 2304: 5.9 / 6.3).
+    int split = 1;
+    if (KIND == E_U8 && !c.offsets && c.K >= 2048) {
+        const int64_t tiles = ((c.M + 127) / 128) * ((c.N + 63) / 64);
+        while (split < 8 && tiles * split * 2 <= (split == 4 ? 64 : 128)) split *= 2;
+    }
+    return launch_blk<KIND, 64>(c, split, stream);
 }
 
 }  // namespace
