@@ -100,11 +100,6 @@ struct BlkArgs {
     int *err;
 };
 
-__device__ __forceinline__ uint4 pack8(bool f16, const float *v) {
-    if (f16) return make_uint4(pack16<true>(v[0], v[1]), pack16<true>(v[2], v[3]), pack16<true>(v[4], v[5]), pack16<true>(v[6], v[7]));
-    return make_uint4(pack16<false>(v[0], v[1]), pack16<false>(v[2], v[3]), pack16<false>(v[4], v[5]), pack16<false>(v[6], v[7]));
-}
-
 __device__ __forceinline__ float silu_fast(float u) { return __fdividef(u, 1.0f + __expf(-u)); }
 
 // Bias of four consecutive columns of group e (zero past N).
@@ -564,6 +559,12 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
         // Gated pairs: chunk c < CPH is g's, chunk c + CPH the same columns of u.
         auto acol = [&](int c) { return NH == 2 ? c * 32 : (c / CPH) * (BN / 2) + (part * CPH + c % CPH) * 32; };
         auto ycol = [&](const Tile &tl, int c) { return (c < CPH ? tl.ocol : tl.b1) + (part * CPH + c % CPH) * 32; };
+        // The bias of this lane's column of a chunk; its row's threads fetch the others' by shuffles (an
+        // address for each of the 128 columns leaves no registers for the sums).
+        auto lane_bias = [&](const Tile &tl, int c) {
+            const int64_t col = (int64_t)ycol(tl, c) + lane;
+            return col < a.N ? __ldg(a.bias + tl.e * a.N + col) : 0.0f;
+        };
         const uint32_t scales = smem_u32(smem) + C::SCALE_OFF;
         for (int t = unit; t < tiles && ok; t += units) {
             if (a.bias && lane < CH && !glu) {  // on its way while the sums are made
@@ -669,7 +670,61 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                 if (!ok) break;
                 boxph ^= 1u;
             }
-            if (wrows > 0 && cta_split == 1) {
+            if constexpr (C::TMA_Y) {
+                if (boxed) {
+                    // 64-column boxes (rows past M and columns past N are clipped): the tile leaves while the
+                    // next one is summed. One branch per step of all chunks: with branches per chunk and word
+                    // this part took 2100 cycles a tile.
+                    if (glu) {
+#pragma unroll
+                        for (int c = 0; c < CPH; ++c)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                acc[c][j].x *= silu_fast(acc[c + CPH][j].x);
+                                acc[c][j].y *= silu_fast(acc[c + CPH][j].y);
+                            }
+                    } else if (a.bias) {
+#pragma unroll
+                        for (int c = 0; c < CH; ++c) {
+                            const float b = lane_bias(tl, c);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                acc[c][j].x += __shfl_sync(0xffffffffu, b, 2 * j);
+                                acc[c][j].y += __shfl_sync(0xffffffffu, b, 2 * j + 1);
+                            }
+                        }
+                    }
+                    if (a.act == 1) {
+#pragma unroll
+                        for (int c = 0; c < CH; ++c)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                acc[c][j].x = fmaxf(acc[c][j].x, 0.0f);
+                                acc[c][j].y = fmaxf(acc[c][j].y, 0.0f);
+                            }
+                    }
+                    uint4 *b = reinterpret_cast<uint4 *>(box) + lane * 8;
+                    auto pack = [&](auto half) {
+                        constexpr bool F16 = decltype(half)::value;
+#pragma unroll
+                        for (int c = 0; c < CH; ++c) {
+                            if (glu && c >= CPH) break;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                b[(c / 2) * 256 + ((4 * (c & 1) + q) ^ (lane & 7))] =
+                                    make_uint4(pack16<F16>(acc[c][4 * q].x, acc[c][4 * q].y),
+                                               pack16<F16>(acc[c][4 * q + 1].x, acc[c][4 * q + 1].y),
+                                               pack16<F16>(acc[c][4 * q + 2].x, acc[c][4 * q + 2].y),
+                                               pack16<F16>(acc[c][4 * q + 3].x, acc[c][4 * q + 3].y));
+                        }
+                    };
+                    if (a.y_dtype == TSFM_DTYPE_F16)
+                        pack(std::true_type{});
+                    else
+                        pack(std::false_type{});
+                }
+            }
+            if (wrows > 0 && cta_split == 1 && !boxed) {
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     if (glu && c >= CPH) break;
@@ -682,24 +737,11 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] *= silu_fast(u[j]);
                     } else if (a.bias) {
-                        // (columns past N, which are not stored, repeat the last one's)
-                        const float *b = a.bias + tl.e * a.N;
-                        const int last = (int)a.N - 1;
+                        const float b = lane_bias(tl, c);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] += __ldg(b + min(col0 + j, last));
+                        for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, b, j);
                     }
-                    if (boxed) {
-                        // 64-column boxes (rows past M and columns past N are clipped): the tile leaves while
-                        // the next one is summed.
-                        if (a.act == 1) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = fmaxf(v[j], 0.0f);
-                        }
-                        const bool f16 = a.y_dtype == TSFM_DTYPE_F16;
-                        uint4 *b = reinterpret_cast<uint4 *>(box) + (c / 2) * 256 + lane * 8;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) b[(4 * (c & 1) + q) ^ (lane & 7)] = pack8(f16, v + 8 * q);
-                    } else if (a.vec32 && col0 + 32 <= a.ycols && !a.accumulate) {
+                    if (a.vec32 && col0 + 32 <= a.ycols && !a.accumulate) {
                         // A thread's 32 columns are whole 32-byte sectors of its row.
                         if (a.act == 1) {
 #pragma unroll
