@@ -18,11 +18,10 @@
 //   warp 2      E4M3, 256 columns: issues the TMA stores of the boxes that the epilogue fills.
 //   warp 3      E4M3: the scales of the tile's rows and columns into a ring of shared memory, four
 //               blocks of K at a time, ahead of the tiles that need them.
-//   warps 4..   epilogue: a thread owns a row and 128 (below 256 columns: 64) of its columns. The
-//               finished sums pass through 4 KB of shared memory a warp, 32 columns at a time, to
-//               row-contiguous stores. That part is kept in small loops: unrolled over the outputs'
-//               types it outgrew the instruction cache, and every step of the kernel took three
-//               times as long.
+//   warps 4..   epilogue: a thread owns a row and 128 (below 256 columns: 64) of its columns, which
+//               are whole 32-byte sectors of y (columns past N, other alignments and sums into y pass
+//               through 4 KB of shared memory a warp). E4M3 on 256 columns with a 16-bit y: through
+//               boxes of 64 columns to TMA stores, so that the tile leaves while the next is summed.
 // E4M3 on 256 columns: each warpgroup of the epilogue has accumulators of its own (two of 128
 // columns), filled by MMAs of its half of the columns, so that handing one back and forth (MMA 256
 // cycles, commit and waits 300, loads 350) takes less than the 1024 cycles that the tensor cores
@@ -30,11 +29,25 @@
 // Rows of a group that end inside a tile: the tile's other rows hold whatever follows in x (or the
 // stage's old bytes), are computed and not stored.
 //
+// What bounds it (B200, 148 SMs, random operands):
+//   16 bits, 256 x 256  the tensor cores: their pipe is active 80 % of the time at M 16384, N 4096,
+//                       K 1024 in 16 groups, 1491 TFLOP/s at M 32768 in 32 groups (184 us).
+//   E4M3, 256 x 256     the epilogue's passes over the accumulators: loads and MMAs alone take 374 ns a
+//                       block of K (3135 TFLOP/s), with the passes 470 ns (K 4096: 278 us for M 75776,
+//                       N 1024, 2282 TFLOP/s); at K 768 a tile's finish is a third (1600 TFLOP/s at
+//                       M 73856, N 2304, 161 us; tensor pipe 38 %). A pass is a chain of waits, tensor-
+//                       memory loads and packed FMAs on two warps per scheduler: 128 sums and 64 loaded
+//                       values a thread leave no room for more warps.
+//   few rows            W's bytes and the start: 32 rows over 24 of 32 experts (N 2048, K 1024) 23 us for
+//                       101 MB in BF16, 20 us for 51 MB in E4M3; one row, N 2304, K 768 6.2 us, of which
+//                       the launch is 2.
+// Tried and slower: 128 x 256 tiles on one SM (their loads alone 526 ns a block of K), 256 x 128 on
+// pairs, 16 epilogue warps of 64 columns (registers spill), test_wait in place of try_wait (2 %).
+//
 // Groups: the offsets are device memory, so the tile list is made on the device: warp 0 scans the
 // groups' row counts into shared memory before the roles start (32 groups a step). Offsets are
 // clamped to [0, M] and to be nondecreasing, so no content of theirs reaches outside x and y.
-// Every element is summed over K by one CTA in a fixed order: no atomics, results do not depend on
-// the grid.
+// Every element is summed over K in a fixed order: no atomics, results do not depend on timing.
 #include "kernels.h"
 #include "ptx.cuh"
 
@@ -179,7 +192,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     constexpr bool SPLIT_REGS = F8 && BN == 256;
     constexpr uint32_t IDESC = idesc_f32acc(KIND == E_BF16 ? 1u : 0u, C::TILE_M, BN / NH);
     const int cta_split = F8 && BN == 64 ? a.split : 1;  // CTAs that share a tile's K
-    const int cta = PAIR ? 2 : cta_split;           // CTAs of a cluster
+    const int cta = PAIR ? 2 : cta_split;                // CTAs of a cluster
     const uint32_t rank = cta > 1 ? cluster_ctarank() : 0u;
     const bool leader = !PAIR || rank == 0;
     const int unit = (int)blockIdx.x / cta, units = (int)gridDim.x / cta;
