@@ -317,8 +317,9 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
  *   [ceil(N / 128), ceil(K / 128)] (row stride ld_ws; one per 128 x 128 block), any FP32 values:
  *   y[m, n] = sum_b x_scale[m, b] w_scale[n / 128, b] sum_{k in block b} x[m, k] W[n, k], sums in
  *   FP32. y_dtype F32, F16 or BF16 (row stride ldy elements, any alignment of the element type);
- *   accumulate (F32 only) adds to y, and the activation then applies to the sum. act: 0 none, 1 relu,
- *   3 gated pairs as in tsfm_kernel_linear (N % 256 == 0, 16-bit y of N / 2 columns, no bias).
+ *   accumulate (F32 only) adds to y, and the activation then applies to the sum. act: 0 none, 1 relu
+ *   (a NaN becomes 0, as in tsfm_kernel_linear), 3 gated pairs as there (N % 256 == 0, 16-bit y of
+ *   N / 2 columns, no bias).
  *   bias [N] or null. M may be 0. y overlaps no input.
  *
  * tsfm_kernel_linear_grouped: y[r] (+)= act(x[r] W[e]^T + bias[e]) for the rows offsets[e] <= r <

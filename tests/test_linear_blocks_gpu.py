@@ -268,6 +268,78 @@ def test_grouped_wide_tiles(kind):
     g.check(torch.float16 if kind == "e4m3" else kind, act=3)
 
 
+# Few rows per group: W's rows as the matrix instruction's, 32 rows of x its columns. Tiles of all four
+# units and of one to three (N 100, 129), K of one block, a ragged quad of blocks and many quads, groups
+# of up to 8 rows, of more, and of more than one tile. Two-byte operands take this way with more tiles
+# than SMs only (groups x N / 128 > 148: the last three).
+FEW = [([1], 64, 64), ([1, 0, 2, 0, 0, 1], 100, 200), ([8, 0, 9, 1, 0, 0, 0], 129, 640), ([0] * 20 + [33, 0, 70], 384, 1300),
+       ([2, 1] * 20, 512, 520), ([0, 1, 3, 0] * 16, 1000, 72), ([1] * 60 + [40, 31, 32], 400, 2056)]
+
+
+@pytest.mark.parametrize("kind", ["e4m3", torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("counts,N,K", FEW, ids=[f"{sum(c)}r{len(c)}g{N}" for c, N, K in FEW])
+def test_grouped_few_rows(kind, counts, N, K):
+    c = Case(sum(counts) + 3, N, K, kind, counts=counts, first=1, bias=True, seed=5)
+    c.check(torch.float32)
+    c.check(torch.bfloat16, act=1)
+    c.check(torch.float16, pad=3, shift=1)
+    c.check(accumulate=1, act=1)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", torch.bfloat16, torch.float16], ids=str)
+def test_grouped_few_rows_gated(kind):
+    for counts, N, K in (([1, 0, 7], 256, 100), ([1, 2] * 40 + [39], 512, 700)):
+        c = Case(sum(counts) + 2, N, K, kind, counts=counts, first=2, seed=6)
+        if kind == "e4m3":
+            k = 0.5 / float(c.ref[c.used].std())
+            c.xs *= k
+            c.ref, c.tol = c.ref * k, 1.1 * c.tol * k  # the scales round again
+        c.check(torch.float16 if kind == "e4m3" else kind, act=3)
+        c.check(torch.bfloat16, act=3, pad=1)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 33, 1), (3, 300, 1024), (8, 5000, 130), (8, 2304, 768)])
+def test_linear_e4m3_few_rows(M, N, K):
+    c = Case(M, N, K, "e4m3", bias=True, seed=7)
+    c.check(torch.float32, pad=5)
+    c.check(torch.bfloat16, act=1)
+    g = Case(M, up(N, 256), K, "e4m3", seed=8)
+    if K > 1:
+        k = 0.5 / float(g.ref.std())
+        g.xs *= k
+        g.ref, g.tol = g.ref * k, 1.1 * g.tol * k
+    g.check(torch.float16, act=3)
+
+
+def test_few_rows_bad_offsets_stay_inside():
+    # negative, falling and far offsets: read as the clamped, nondecreasing ones
+    M = 20
+    c = Case(M, 96, 200, "e4m3", counts=[6, 0, 14, 0])
+    off = torch.tensor([-50, 6, 4, 2 ** 31 - 1, 3], dtype=torch.int32, device="cuda")
+    a, b = torch.full((M + 64, 96), 3.0, device="cuda"), torch.full((M + 64, 96), 3.0, device="cuda")
+    tb.check(c.call(a))
+    tb.check(c.call(b, off=off))
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and (a[:M] != 3.0).any() and (b[M:] == 3.0).all()
+
+
+def test_few_rows_nonfinite_values():
+    # a row of NaN beside others of its tile, an infinite scale, a weight block of NaN scale: only what
+    # they belong to shows them
+    c = Case(12, 256, 512, "e4m3", counts=[5, 0, 7], seed=9)
+    c.x[2, 7] = float("nan")
+    c.xs[6, 1] = float("inf")
+    c.ws[2, 1, 0] = float("nan")  # columns 128.. of the last group
+    y = torch.zeros(12, 256, device="cuda")
+    tb.check(c.call(y))
+    torch.cuda.synchronize()
+    ok = ((y.double() - c.ref).abs() <= c.tol + (c.ref.abs() + c.tol) * 2.0 ** -24)
+    assert torch.isnan(y[2]).all() and not torch.isfinite(y[6]).any()
+    assert torch.isnan(y[5:, 128:]).all()
+    assert ok[[0, 1, 3, 4]].all() and ok[[5, 7, 8, 9, 10, 11]][:, :128].all()
+
+
+
 def test_linear_e4m3_offsets_past_32_bits():
     # y of more than 2^31 elements and x of more than 2^31 bytes: the last rows and columns
     M, N, K = 140000, 16384, 16400

@@ -38,11 +38,10 @@
 //                       M 73856, N 2304, 161 us; tensor pipe 38 %). A pass is a chain of waits, tensor-
 //                       memory loads and packed FMAs on two warps per scheduler: 128 sums and 64 loaded
 //                       values a thread leave no room for more warps.
-//   few rows            W's bytes and the start: 32 rows over 24 of 32 experts (N 2048, K 1024) 23 us for
-//                       101 MB in BF16, 20 us for 51 MB in E4M3; one row, N 2304, K 768 6.2 us, of which
-//                       the launch is 2.
-// Tried and slower: 128 x 256 tiles on one SM (their loads alone 526 ns a block of K), 256 x 128 on
-// pairs, 16 epilogue warps of 64 columns (registers spill), test_wait in place of try_wait (2 %).
+//   few rows            the start and W's bytes; groups of few rows have a kernel of their own below.
+// Tried and slower: 128 x 256 tiles on one SM (their loads alone 526 ns a block of K), there also 16
+// epilogue warps of 64 columns (registers spill; 401 ns against 377 for 8 warps), test_wait in place of
+// try_wait (2 %).
 //
 // Groups: the offsets are device memory, so the tile list is made on the device: warp 0 scans the
 // groups' row counts into shared memory before the roles start (32 groups a step). Offsets are
@@ -99,6 +98,7 @@ struct BlkArgs {
     int64_t M, N, K;
     const int32_t *offsets;
     int groups, n_tiles, num_k;
+    uint32_t n_inv;  // (2^32 - 1) / n_tiles
     const float *xs, *ws;
     int64_t ld_xs, ld_ws, ws_group;
     int ws_blocks;  // blocks of N
@@ -179,6 +179,80 @@ __device__ __forceinline__ void store_sectors(void *o, const float (&v)[32]) {
     }
 }
 
+// The groups' rows and tiles of TILE_M rows, by one warp: group e has rows [g_row[e], g_row[e + 1]) and
+// row tiles [g_tile[e], g_tile[e + 1]). No offsets: one group of M rows.
+// `first` and `o` (a lane's first offset) are loaded before, so that they are on their way while the
+// barriers are initialised. All that runs before the first load of an operand runs once per launch, from
+// instructions that no cache of the SM holds yet: about 30 cycles each, so loops stay rolled (unrolled,
+// the two scans took 2.5 us) and divisions are by reciprocals from the host.
+template <int TILE_M>
+__device__ __forceinline__ void scan_groups(const BlkArgs &a, int lane, int first, int o, int *g_row, int *g_tile) {
+    if (a.offsets == nullptr) {
+        if (lane == 0) {
+            g_row[0] = g_tile[0] = 0;
+            g_row[1] = (int)a.M;
+            g_tile[1] = (int)((a.M + TILE_M - 1) / TILE_M);
+        }
+        return;
+    }
+    const int M = (int)a.M;
+    int end = min(max(first, 0), M);  // running maximum of the offsets
+    int tiles = 0;
+    if (lane == 0) {
+        g_row[0] = end;
+        g_tile[0] = 0;
+    }
+    for (int base = 0; base < a.groups; base += 32) {
+        const int e = base + lane;
+        o = max(min(max(o, 0), M), end);
+#pragma unroll 1
+        for (int d = 1; d < 32; d <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, o, d);
+            if (lane >= d) o = max(o, p);
+        }
+        int start = __shfl_up_sync(0xffffffffu, o, 1);
+        if (lane == 0) start = end;
+        int t = (o - start + TILE_M - 1) / TILE_M;
+#pragma unroll 1
+        for (int d = 1; d < 32; d <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, t, d);
+            if (lane >= d) t += p;
+        }
+        if (e < a.groups) {
+            g_row[e + 1] = o;
+            g_tile[e + 1] = tiles + t;
+        }
+        end = __shfl_sync(0xffffffffu, o, 31);
+        tiles += __shfl_sync(0xffffffffu, t, 31);
+        o = e + 32 < a.groups ? __ldg(a.offsets + e + 33) : 0;
+    }
+}
+
+// Tile t of n_tiles per row tile: its row tile (returned) and the rest. The product with n_inv is short
+// of t / n_tiles by less than one.
+__device__ __forceinline__ int split_tile(const BlkArgs &a, int t, int &nt) {
+    int mt = (int)__umulhi((uint32_t)t, a.n_inv);
+    nt = t - mt * a.n_tiles;
+    if (nt >= a.n_tiles) {
+        nt -= a.n_tiles;
+        ++mt;
+    }
+    return mt;
+}
+
+// The group of row tile mt: the last e with g_tile[e] <= mt.
+__device__ __forceinline__ int group_of(const int *g_tile, int groups, int mt) {
+    int lo = 0, hi = groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (g_tile[mid] <= mt)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
 template <int KIND, int BN>
 __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     linear_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -217,69 +291,23 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (threadIdx.x == 64) {
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        for (int i = 0; i < NH * NBUF; ++i) {
-            mbar_init(&pfull[i], 1);
-            mbar_init(&pempty[i], (PAIR ? 2 : 1) * C::EPI_WARPS / NH);  // one arrival per epilogue warp
-        }
-        for (int i = 0; i < C::EPI_WARPS; ++i) {
-            mbar_init(&bfull[i], 1);
-            mbar_init(&bempty[i], 1);
-        }
-        for (int i = 0; i < kScaleSlots; ++i) {
-            mbar_init(&sfull[i], 32);
-            mbar_init(&sempty[i], C::EPI_WARPS);
-        }
-        mbar_init(drain, 1);
-        *abort_flag = 0;
+    if (warp == 2) {
+        for (uint64_t *b = full + lane; b <= drain; b += 32)
+            mbar_init(b, b >= pempty && b < sfull    ? (PAIR ? 2 : 1) * C::EPI_WARPS / NH  // one arrival per epilogue warp
+                         : b >= sfull && b < sempty  ? 32
+                         : b >= sempty && b < bfull  ? C::EPI_WARPS
+                                                     : 1);
+        if (lane == 0) *abort_flag = 0;
         fence_barrier_init();
-        tma_prefetch_desc(&tmA);
-        tma_prefetch_desc(&tmB);
     }
-    if (warp == 0 && a.offsets == nullptr) {
+    if (warp == 0) {
+        const int first = a.offsets ? __ldg(a.offsets) : 0;
+        const int o = a.offsets && lane < a.groups ? __ldg(a.offsets + lane + 1) : 0;
         if (lane == 0) {
-            g_row[0] = g_tile[0] = 0;
-            g_row[1] = (int)a.M;
-            g_tile[1] = (int)((a.M + C::TILE_M - 1) / C::TILE_M);
+            tma_prefetch_desc(&tmA);
+            tma_prefetch_desc(&tmB);
         }
-    } else if (warp == 0) {
-        const int M = (int)a.M;
-        const int first = __ldg(a.offsets);
-        int o = lane < a.groups ? __ldg(a.offsets + lane + 1) : 0;
-        int end = min(max(first, 0), M);  // running maximum of the offsets
-        int tiles = 0;
-        if (lane == 0) {
-            g_row[0] = end;
-            g_tile[0] = 0;
-        }
-        for (int base = 0; base < a.groups; base += 32) {
-            const int e = base + lane;
-            o = max(min(max(o, 0), M), end);
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int p = __shfl_up_sync(0xffffffffu, o, d);
-                if (lane >= d) o = max(o, p);
-            }
-            int start = __shfl_up_sync(0xffffffffu, o, 1);
-            if (lane == 0) start = end;
-            int t = (o - start + C::TILE_M - 1) / C::TILE_M;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int p = __shfl_up_sync(0xffffffffu, t, d);
-                if (lane >= d) t += p;
-            }
-            if (e < a.groups) {
-                g_row[e + 1] = o;
-                g_tile[e + 1] = tiles + t;
-            }
-            end = __shfl_sync(0xffffffffu, o, 31);
-            tiles += __shfl_sync(0xffffffffu, t, 31);
-            o = e + 32 < a.groups ? __ldg(a.offsets + e + 33) : 0;
-        }
+        scan_groups<C::TILE_M>(a, lane, first, o, g_row, g_tile);
     }
     if (warp == 1) {
         __syncwarp();
@@ -306,16 +334,9 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     const bool glu = a.act == ACT_GLU;
     auto tile_at = [&](int t) {
         Tile r;
-        const int mt = t / a.n_tiles, nt = t - mt * a.n_tiles;
-        int lo = 0, hi = a.groups - 1;  // the last e with g_tile[e] <= mt
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (g_tile[mid] <= mt)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        r.e = lo;
+        int nt;
+        const int mt = split_tile(a, t, nt);
+        const int lo = r.e = group_of(g_tile, a.groups, mt);
         r.row0 = g_row[lo] + (mt - g_tile[lo]) * C::TILE_M + (PAIR ? (int)rank * 128 : 0);
         r.row_end = g_row[lo + 1];
         if (glu) {
@@ -846,35 +867,367 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     if constexpr (PAIR) cluster_sync_all();
 }
 
-// split: CTAs that share a tile's K (64-wide E4M3 tiles; one tile per cluster, the grid covers every tile).
-template <int KIND, int BN>
-Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
-    using C = BlkCfg<KIND, BN>;
-    constexpr bool PAIR = C::PAIR;
-    constexpr int BK = C::F8 ? 128 : 64;
-    alignas(64) CUtensorMap ta, tb, ty;
-    const bool glu = c.act == ACT_GLU;
-    {
-        const int64_t d[2] = {c.K, c.M}, st[2] = {1, c.ldx};
-        const uint32_t box[2] = {BK, C::A_BOX};
-        TSFM_TRY(make_tmap_nd(&ta, c.x, KIND, 2, d, st, box));
+// Few rows per group (serving: some tokens over many experts, each W read for a row or two): the
+// operands change places. W's rows are the MMA's 128 rows and 32 rows of x its columns, so that a block
+// of K costs the epilogue 8 or 32 sums a thread instead of 64, and a thread owns one output column.
+// CTAs take tiles of 128 rows of W (four units of 32, one per epilogue warp; gated pairs: 16 rows of g
+// and the 16 of u) by 32 rows of x in turn. Tiles of fewer units, to share the last round evenly, were
+// slower: what an SM receives is its share of the bytes under way, and 200 KB a CTA keep HBM busy through
+// a round that not all SMs have. Loads start before the block has met.
+// Bound by W's bytes and the start. 32 rows over 24 of 32 groups, N 2048, K 1024: E4M3 13.4 us for 51 MB
+// (3.8 TB/s; the first load is issued after 2.2 us, the last has landed after 11 to 12.3), BF16 21.9 us
+// for 101 MB (4.6 TB/s); 128-wide tiles take 19.6 and 23.3.
+//   warp 0  offsets, TMA producer        warp 1  tensor memory, MMA issue
+//   warp 3  E4M3: scales                 warps 4..7  epilogue, one unit each
+template <int KIND>
+struct FewCfg {
+    static constexpr bool F8 = KIND == E_U8;
+    static constexpr int ROWS = 32, THREADS = 256, STAGES = 10;
+    static constexpr int W_BYTES = 128 * 128, X_BYTES = ROWS * 128, UNIT_BYTES = 32 * 128;
+    static constexpr int NBUF = 2;  // accumulators: one per tile, or (E4M3) one per quad of blocks of K, four parts
+    static constexpr int ACC_COLS = F8 ? kScaleQuad * ROWS : ROWS;
+    static constexpr int TMEM_COLS = NBUF * ACC_COLS;
+    static constexpr int SLOTS = 8, SLOT_BYTES = kScaleQuad * (ROWS + 8) * 4;  // xs[block][row], then ws[unit][2][block]
+    static constexpr int SCALE_OFF = STAGES * (W_BYTES + X_BYTES);
+    static constexpr int BAR_OFF = SCALE_OFF + (F8 ? SLOTS * SLOT_BYTES : 0);
+    static constexpr int GROUP_OFF = BAR_OFF + 512;
+    static int smem(int64_t groups) { return 1024 + GROUP_OFF + 8 * (int)(groups + 1); }
+    static_assert((2 * STAGES + 2 * NBUF + 2 * SLOTS + 2) * 8 <= 512, "barriers");
+};
+
+template <int KIND>
+__global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
+    linear_few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                           const __grid_constant__ CUtensorMap tmW4, BlkArgs a) {
+    using C = FewCfg<KIND>;
+    constexpr bool F8 = C::F8;
+    constexpr int STAGES = C::STAGES, NBUF = C::NBUF, SLOTS = C::SLOTS;
+    constexpr int BK = F8 ? 128 : 64;
+    constexpr uint32_t IDESC = idesc_f32acc(KIND == E_BF16 ? 1u : 0u, 128, C::ROWS);
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sW = smem;
+    uint8_t *sX = smem + STAGES * C::W_BYTES;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);
+    uint64_t *empty = full + STAGES;
+    uint64_t *pfull = empty + STAGES;
+    uint64_t *pempty = pfull + NBUF;
+    uint64_t *sfull = pempty + NBUF;
+    uint64_t *sempty = sfull + SLOTS;
+    uint64_t *drain = sempty + SLOTS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    int *g_row = reinterpret_cast<int *>(smem + C::GROUP_OFF);
+    int *g_tile = g_row + a.groups + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool glu = a.act == ACT_GLU;
+
+    struct Tile {
+        int e, row0, rows;  // group, first row of x, rows (at most 32)
+        int n0, cnt;        // first unit of W, units (at most 4)
+    };
+    auto tile_at = [&](int t) {
+        Tile r;
+        int nt;
+        const int mt = split_tile(a, t, nt);
+        r.n0 = nt * 4;
+        r.cnt = min(4, (int)((a.N + 31) >> 5) - r.n0);
+        r.e = group_of(g_tile, a.groups, mt);
+        r.row0 = g_row[r.e] + (mt - g_tile[r.e]) * C::ROWS;
+        r.rows = min(C::ROWS, g_row[r.e + 1] - r.row0);
+        return r;
+    };
+    auto tiles = [&]() { return g_tile[a.groups] * a.n_tiles; };  // the host has checked that this fits
+    auto wait = [&](uint64_t *bar, uint32_t parity, int site) {
+        return mbar_wait_warp(bar, parity, abort_flag, a.err, site);
+    };
+
+    if (warp == 0) {
+        const int first = a.offsets ? __ldg(a.offsets) : 0;
+        const int o = a.offsets && lane < a.groups ? __ldg(a.offsets + lane + 1) : 0;
+        if (lane == 0) {
+            tma_prefetch_desc(&tmX);
+            tma_prefetch_desc(glu ? &tmW : &tmW4);
+            *abort_flag = 0;
+        }
+        for (uint64_t *b = full + lane; b <= drain; b += 32)
+            mbar_init(b, (b >= pempty && b < sfull) || (b >= sempty && b < drain) ? 4 : b >= sfull && b < sempty ? 32 : 1);
+        fence_barrier_init();
+        scan_groups<C::ROWS>(a, lane, first, o, g_row, g_tile);
+        __syncwarp();
+        // The first use of each stage waits for nothing and comes before the block has met.
+        const bool el = elect_one();
+        int s = 0, i = 0;
+        uint32_t ph = 0, issued = 0, issued_ph = 0;
+        bool ok = true, met = false;
+        for (int t = (int)blockIdx.x; t < tiles() && ok; t += (int)gridDim.x) {
+            const Tile tl = tile_at(t);
+            for (int kb = 0; kb < a.num_k; ++kb) {
+                if (i == STAGES && !met) {
+                    __syncthreads();
+                    met = true;
+                }
+                if (met) {
+                    ok = wait(&empty[s], ph ^ 1u, ERR_SITE_BLOCKS_PRODUCER);
+                    if (!ok) break;
+                }
+                const int32_t kc = kb * BK;
+                if (el) {
+                    mbar_arrive_expect_tx(&full[s], tl.cnt * C::UNIT_BYTES + C::X_BYTES);
+                    if (tl.cnt == 4 && !glu)  // whole tiles in one copy
+                        tma_load_5d(sW + s * C::W_BYTES, &tmW4, &full[s], kc, tl.n0 * 32, 0, 0, tl.e);
+                    for (int n = tl.cnt == 4 && !glu ? 4 : 0; n < tl.cnt; ++n) {
+                        const int first = (tl.n0 + n) * (glu ? 16 : 32);
+                        tma_load_5d(sW + s * C::W_BYTES + n * C::UNIT_BYTES, &tmW, &full[s], kc, glu ? first & 127 : first, 0,
+                                    glu ? first >> 7 : 0, tl.e);
+                    }
+                    tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], kc, tl.row0);
+                }
+                __syncwarp();
+                issued |= 1u << s;
+                issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
+                i += !met;
+                if (++s == STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        if (!met) __syncthreads();
+        if (!ok) {
+            // Loads in flight land before the CTA can exit (bounded).
+            const unsigned long long t0 = globaltimer_ns();
+            for (int k = 0; k < STAGES; ++k) {
+                if (!((issued >> k) & 1u)) continue;
+                while (!mbar_try_wait(&full[k], (issued_ph >> k) & 1u) && globaltimer_ns() - t0 < 100000000ull) {
+                }
+            }
+        }
+    } else {
+        if (warp == 1) {
+            tmem_alloc(tmem_slot, C::TMEM_COLS);
+            tmem_relinquish();
+            tc_fence_before();
+        }
+        __syncthreads();
+        tc_fence_after();
     }
-    {
-        // W [groups, N, K]; for gated pairs [groups, N / 256, 2, 128, K].
-        const int64_t wg = c.groups > 1 ? c.w_group : c.N * c.ldw;
-        const int64_t d[5] = {c.K, glu ? 128 : c.N, glu ? 2 : 1, glu ? c.N / 256 : 1, c.groups};
-        const int64_t st[5] = {1, c.ldw, glu ? 128 * c.ldw : c.N * c.ldw, glu ? 256 * c.ldw : c.N * c.ldw, wg};
-        const uint32_t box[5] = {BK, (uint32_t)(PAIR || glu ? BN / 2 : BN), !PAIR && glu ? 2u : 1u, 1, 1};
-        TSFM_TRY(make_tmap_nd(&tb, c.w, KIND, 5, d, st, box));
+    const uint32_t tmem_base = warp == 0 ? 0u : *tmem_slot;
+
+    if (warp == 1) {
+        const bool el = elect_one();
+        int s = 0, buf = 0;
+        uint32_t ph = 0, bph = 0;
+        bool ok = true;
+        const uint64_t wd0 = sdesc_k128(sW), xd0 = sdesc_k128(sX);
+        for (int t = (int)blockIdx.x; t < tiles() && ok; t += (int)gridDim.x) {
+            for (int kb = 0; kb < a.num_k; ++kb) {
+                ok = wait(&full[s], ph, ERR_SITE_BLOCKS_MMA_FULL);
+                if (ok && (F8 ? kb % kScaleQuad : kb) == 0) ok = wait(&pempty[buf], bph ^ 1u, ERR_SITE_BLOCKS_MMA_EMPTY);
+                if (!ok) break;
+                tc_fence_after();
+                const bool last = kb == a.num_k - 1 || (F8 && kb % kScaleQuad == kScaleQuad - 1);
+                if (el) {
+                    const uint64_t wd = wd0 + (uint64_t)(s * (C::W_BYTES >> 4)), xd = xd0 + (uint64_t)(s * (C::X_BYTES >> 4));
+                    const uint32_t d = tmem_base + (uint32_t)(buf * C::ACC_COLS + (F8 ? kb % kScaleQuad * C::ROWS : 0));
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        if constexpr (F8)
+                            mma_f8kind(d, wd + 2 * kk, xd + 2 * kk, IDESC, kk != 0);
+                        else
+                            mma_f16kind(d, wd + 2 * kk, xd + 2 * kk, IDESC, (kb | kk) != 0);
+                    }
+                    if (last) mma_commit(&pfull[buf]);
+                    mma_commit(&empty[s]);
+                }
+                __syncwarp();
+                if (last && ++buf == NBUF) {
+                    buf = 0;
+                    bph ^= 1u;
+                }
+                if (++s == STAGES) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        // All MMAs issued by this warp have completed once `drain` fires (also on the abort path).
+        if (el) {
+            mma_commit(drain);
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try_wait(drain, 0)) {
+                if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+                    if (a.err) atomicCAS(a.err, 0, ERR_SITE_BLOCKS_DRAIN);
+                    break;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (F8 && warp == 3) {
+        int slot = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int t = (int)blockIdx.x; t < tiles() && ok; t += (int)gridDim.x) {
+            const Tile tl = tile_at(t);
+            const float *xs = a.xs + (int64_t)(tl.row0 + min(lane, tl.rows - 1)) * a.ld_xs;  // the last row's again past the end
+            // lane = (unit, half of a gated unit, block of K)
+            const int first = (tl.n0 + (lane >> 3)) * (glu ? 16 : 32);
+            const int nb = glu ? (first >> 7) * 2 + ((lane >> 2) & 1) : first >> 7;
+            const float *ws = a.ws + tl.e * a.ws_group + (int64_t)min(nb, a.ws_blocks - 1) * a.ld_ws + (lane & 3);
+            for (int kb = 0; kb < a.num_k; kb += kScaleQuad) {
+                ok = wait(&sempty[slot], ph ^ 1u, ERR_SITE_BLOCKS_PRODUCER);
+                if (!ok) break;
+                uint8_t *d = smem + C::SCALE_OFF + slot * C::SLOT_BYTES;
+                const int n = min(kScaleQuad, a.num_k - kb);
+                for (int j = 0; j < n; ++j) cp_async_4(d + (j * C::ROWS + lane) * 4, xs + kb + j);
+                if ((lane & 3) < n) cp_async_4(d + kScaleQuad * C::ROWS * 4 + lane * 4, ws + kb);
+                cp_async_arrive(&sfull[slot]);
+                if (++slot == SLOTS) {
+                    slot = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        cp_async_wait_all();
+    } else if (warp >= 4) {
+        const int unit = warp & 3;  // of the tile; tensor-memory lanes [32 unit, 32 unit + 32)
+        int buf = 0, slot = 0;
+        uint32_t bph = 0, sph = 0;
+        bool ok = true;
+        auto release = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pempty[buf]);
+            if (++buf == NBUF) {
+                buf = 0;
+                bph ^= 1u;
+            }
+        };
+        const uint32_t scales = smem_u32(smem) + C::SCALE_OFF;
+        for (int t = (int)blockIdx.x; t < tiles() && ok; t += (int)gridDim.x) {
+            const Tile tl = tile_at(t);
+            const bool mine = unit < tl.cnt;
+            const int col = glu ? (tl.n0 + unit) * 16 + (lane & 15) : (tl.n0 + unit) * 32 + lane;
+            const bool out = mine && col < a.ycols && (!glu || lane < 16);
+            const float bias = out && a.bias ? __ldg(a.bias + tl.e * a.N + col) : 0.0f;
+            float v[32];
+            auto tbase = [&]() { return tmem_base + ((uint32_t)(unit * 32) << 16) + (uint32_t)(buf * C::ACC_COLS); };
+            if constexpr (F8) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                for (int kb = 0; kb < a.num_k && ok; kb += kScaleQuad) {
+                    ok = wait(&sfull[slot], sph, ERR_SITE_BLOCKS_EPILOGUE) && wait(&pfull[buf], bph, ERR_SITE_BLOCKS_EPILOGUE);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sc = scales + slot * C::SLOT_BYTES;
+                    const int n = min(kScaleQuad, a.num_k - kb);
+                    // Four blocks of K a hand-over: one at a time, its waits and loads took 420 cycles each.
+                    auto add = [&](auto count) {
+                        constexpr int R = decltype(count)::value;
+                        float p[kScaleQuad][R], w[4];
+#pragma unroll
+                        for (int j = 0; j < kScaleQuad; ++j) {
+                            if constexpr (R == 32)
+                                tmem_ld32f(tbase() + j * C::ROWS, p[j]);
+                            else
+                                tmem_ld8f(tbase() + j * C::ROWS, p[j]);
+                        }
+                        ld_shared_v4(sc + kScaleQuad * C::ROWS * 4 + (unit * 2 + (lane >> 4)) * 16, w);
+                        tmem_wait_ld();
+                        release();
+#pragma unroll
+                        for (int j = 0; j < kScaleQuad; ++j) {
+                            if (j >= n) break;
+#pragma unroll
+                            for (int q = 0; q < R / 4; ++q) {
+                                float x[4];
+                                ld_shared_v4(sc + (j * C::ROWS + 4 * q) * 4, x);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[4 * q + i] = fmaf(p[j][4 * q + i], w[j] * x[i], v[4 * q + i]);
+                            }
+                        }
+                    };
+                    if (!mine)
+                        release();
+                    else if (tl.rows <= 8)
+                        add(std::integral_constant<int, 8>{});
+                    else
+                        add(std::integral_constant<int, 32>{});
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[slot]);
+                    if (++slot == SLOTS) {
+                        slot = 0;
+                        sph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+            } else {
+                ok = wait(&pfull[buf], bph, ERR_SITE_BLOCKS_EPILOGUE);
+                if (!ok) break;
+                tc_fence_after();
+                tmem_ld32f(tbase(), v);
+                tmem_wait_ld();
+                release();
+            }
+            if (!mine) continue;
+            if (glu) {
+#pragma unroll
+                for (int r = 0; r < 32; ++r) {
+                    if (r >= tl.rows) break;
+                    v[r] *= silu_fast(__shfl_xor_sync(0xffffffffu, v[r], 16));
+                }
+            }
+            auto store = [&](auto type) {
+                using T = decltype(type);
+                T *y = static_cast<T *>(a.y) + (int64_t)tl.row0 * a.ldy + col;
+#pragma unroll
+                for (int r = 0; r < 32; ++r) {
+                    if (r >= tl.rows) break;
+                    float f = v[r] + bias;
+                    if (out) {
+                        if constexpr (std::is_same<T, float>::value) {
+                            if (a.accumulate) f += *y;
+                        }
+                        if (a.act == 1) f = fmaxf(f, 0.0f);
+                        if constexpr (std::is_same<T, float>::value)
+                            *y = f;
+                        else if constexpr (std::is_same<T, __half>::value)
+                            *y = __float2half_rn(f);
+                        else
+                            *y = __float2bfloat16_rn(f);
+                    }
+                    y += a.ldy;
+                }
+            };
+            if (a.y_dtype == TSFM_DTYPE_F32)
+                store(float{});
+            else if (a.y_dtype == TSFM_DTYPE_F16)
+                store(__half{});
+            else
+                store(__nv_bfloat16{});
+        }
     }
-    BlkArgs a;
+
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+}
+
+BlkArgs blk_args(const LinearBlocksCall &c, int n_tiles, int bk) {
+    BlkArgs a = {};
     a.M = c.M;
     a.N = c.N;
     a.K = c.K;
     a.offsets = c.offsets;
     a.groups = (int)c.groups;
-    a.n_tiles = (int)((c.N + BN - 1) / BN);
-    a.num_k = (int)((c.K + BK - 1) / BK);
+    a.n_tiles = n_tiles;
+    a.n_inv = 0xffffffffu / (uint32_t)n_tiles;
+    a.num_k = (int)((c.K + bk - 1) / bk);
     a.xs = c.xs;
     a.ws = c.ws;
     a.ld_xs = c.ld_xs;
@@ -884,10 +1237,63 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     a.bias = c.bias;
     a.y = c.y;
     a.ldy = c.ldy;
-    a.ycols = glu ? c.N / 2 : c.N;
+    a.ycols = c.act == ACT_GLU ? c.N / 2 : c.N;
     a.y_dtype = c.y_dtype;
     a.accumulate = c.accumulate;
     a.act = c.act;
+    a.err = c.err;
+    return a;
+}
+
+// x by boxes of `rows` rows and W [groups, N, K] by boxes of w_rows rows; for gated pairs W is [groups,
+// N / 256, 2, 128, K] and a box holds w_rows rows of each of w_halves of them.
+Status operand_maps(const LinearBlocksCall &c, int kind, uint32_t bk, uint32_t rows, uint32_t w_rows, uint32_t w_halves,
+                    CUtensorMap *tx, CUtensorMap *tw) {
+    const bool glu = c.act == ACT_GLU;
+    const int64_t dx[2] = {c.K, c.M}, sx[2] = {1, c.ldx};
+    const uint32_t bx[2] = {bk, rows};
+    TSFM_TRY(make_tmap_nd(tx, c.x, kind, 2, dx, sx, bx));
+    const int64_t wg = c.groups > 1 ? c.w_group : c.N * c.ldw;
+    const int64_t dw[5] = {c.K, glu ? 128 : c.N, glu ? 2 : 1, glu ? c.N / 256 : 1, c.groups};
+    const int64_t sw[5] = {1, c.ldw, glu ? 128 * c.ldw : c.N * c.ldw, glu ? 256 * c.ldw : c.N * c.ldw, wg};
+    const uint32_t bw[5] = {bk, w_rows, w_halves, 1, 1};
+    return make_tmap_nd(tw, c.w, kind, 5, dw, sw, bw);
+}
+
+// At most this many tiles of `rows` rows: every group may end inside one.
+int64_t most_row_tiles(const LinearBlocksCall &c, int rows) {
+    return c.offsets ? c.M / rows + std::min(c.groups, c.M) : (c.M + rows - 1) / rows;
+}
+
+template <int KIND>
+Status launch_few(const LinearBlocksCall &c, cudaStream_t stream) {
+    using C = FewCfg<KIND>;
+    constexpr int BK = C::F8 ? 128 : 64;
+    alignas(64) CUtensorMap tx, tw, tw4;
+    const bool glu = c.act == ACT_GLU;
+    TSFM_TRY(operand_maps(c, KIND, BK, C::ROWS, glu ? 16 : 32, glu ? 2 : 1, &tx, &tw));
+    tw4 = tw;
+    if (!glu) TSFM_TRY(operand_maps(c, KIND, BK, C::ROWS, 128, 1, &tx, &tw4));
+    const BlkArgs a = blk_args(c, (int)((c.N + 127) / 128), BK);
+    const int smem = C::smem(c.groups);
+    TSFM_TRY(ensure_smem_attr(reinterpret_cast<const void *>(&linear_few_rows_kernel<KIND>), smem));
+    const int64_t most = most_row_tiles(c, C::ROWS) * a.n_tiles;
+    if (most > INT32_MAX / 16) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: too many tiles");
+    linear_few_rows_kernel<KIND><<<(unsigned)std::min<int64_t>(most, num_sms()), C::THREADS, smem, stream>>>(tx, tw, tw4, a);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? Status::ok() : Status::cuda(e, "linear (few rows): launch");
+}
+
+// split: CTAs that share a tile's K (64-wide E4M3 tiles; one tile per cluster, the grid covers every tile).
+template <int KIND, int BN>
+Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
+    using C = BlkCfg<KIND, BN>;
+    constexpr bool PAIR = C::PAIR;
+    constexpr int BK = C::F8 ? 128 : 64;
+    alignas(64) CUtensorMap ta, tb, ty;
+    const bool glu = c.act == ACT_GLU;
+    TSFM_TRY(operand_maps(c, KIND, BK, C::A_BOX, PAIR || glu ? BN / 2 : BN, !PAIR && glu ? 2 : 1, &ta, &tb));
+    BlkArgs a = blk_args(c, (int)((c.N + BN - 1) / BN), BK);
     const int ysz = c.y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
     a.vec = reinterpret_cast<uintptr_t>(c.y) % (4 * ysz) == 0 && c.ldy % 4 == 0;
     a.vec32 = reinterpret_cast<uintptr_t>(c.y) % 32 == 0 && (c.ldy * ysz) % 32 == 0;
@@ -899,13 +1305,10 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
         TSFM_TRY(make_tmap_nd(&ty, c.y, c.y_dtype == TSFM_DTYPE_F16 ? E_F16 : E_BF16, 2, d, st, box));
     }
     a.split = split;
-    a.err = c.err;
     const int smem = C::smem(c.groups);
     const void *fn = reinterpret_cast<const void *>(&linear_blocks_kernel<KIND, BN>);
     TSFM_TRY(ensure_smem_attr(fn, smem));
-    // At most this many row tiles: every group may end inside one.
-    const int64_t row_tiles = c.offsets ? c.M / C::TILE_M + std::min(c.groups, c.M) : (c.M + C::TILE_M - 1) / C::TILE_M;
-    const int64_t most = row_tiles * a.n_tiles;
+    const int64_t most = most_row_tiles(c, C::TILE_M) * a.n_tiles;
     if (most > INT32_MAX / 16) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: too many tiles");
     const int cta = PAIR ? 2 : split;
     cudaLaunchConfig_t cfg = {};
@@ -959,8 +1362,27 @@ int tile_width(const LinearBlocksCall &c) {
     return best;
 }
 
+// Whether a call's groups are taken to have few rows. Measured, us on 64- or 128-wide tiles / with the
+// operands exchanged:
+//   E4M3, N 2048 K 1024, 32 groups:  M 32 19.6 / 13.4   M 192 19.6 / 14.9   M 256 (gated) 17.0 / 20.1
+//     all rows in one group:         M 32  8.1 /  8.8   M 128  8.8 /  8.9
+//     4 groups:                      M  4  7.4 /  7.2   M  32  7.5 /  8.1
+//   BF16, the same, 32 groups:       M 32 23.3 / 21.9   M 192 24.1 / 22.6   M 256 (gated) 23.5 / 25.1
+//     4 groups (fewer tiles than SMs, where nothing waits for memory): M 4 8.6 / 9.7
+//   E4M3, one product (N 2304 K 768): M 1 6.4 / 5.8      M 8 6.4 / 6.2       M 16 6.3 / 6.8
+//     K 4096, which a cluster's CTAs share on 64-wide tiles (N 1024): M 1 7.5 / 13.2
+// The host does not know the groups' rows. Rows spread over 192 of 256 groups (M 1536, N 1024, K 512,
+// E4M3) take 50.4 / 30.5, all of them in one group 11.6 / 17.8: the loss is smaller than the gain.
+template <int KIND>
+bool few_rows(const LinearBlocksCall &c) {
+    const bool f8 = KIND == E_U8;
+    if (!c.offsets) return f8 && c.M <= 8 && c.K <= 1024;
+    return c.M <= 6 * c.groups && (f8 || std::min(c.groups, c.M) * ((c.N + 127) / 128) > num_sms());
+}
+
 template <int KIND>
 Status launch_kind(const LinearBlocksCall &c, cudaStream_t stream) {
+    if (few_rows<KIND>(c)) return launch_few<KIND>(c, stream);
     const int bn = tile_width<KIND>(c);
     if (bn == 256) return launch_blk<KIND, 256>(c, 1, stream);
     if (bn == 128) return launch_blk<KIND, 128>(c, 1, stream);
