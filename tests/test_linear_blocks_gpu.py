@@ -533,3 +533,52 @@ def test_feed_forward_chain():
         assert ((y[lo:hi].double() - hv[lo:hi] @ w.T).abs() <= tol).all()
     # quantising is off by at most half an E4M3 step of the block's grid
     assert ((xv - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * xs.double().repeat_interleave(128, 1)).all()
+
+
+@pytest.mark.parametrize("M", [5, 300, 3000])
+def test_back_to_back_calls_see_their_predecessors(M):
+    # Calls that read what the call before wrote and overwrite what it read, without a pause between
+    # them, eager and captured, against the same calls one at a time.
+    G, D = 4, 512
+    g = gen(M)
+    wq, ws = quantize(torch.randn(G * D, D, generator=g, device="cuda") * 1.4 * D ** -0.5, 128)
+    w16 = (torch.randn(G, D, D, generator=g, device="cuda") * 1.4 * D ** -0.5).bfloat16()
+    off = torch.tensor([0, M // 3, M // 3, M - 1, M], dtype=torch.int32, device="cuda")
+    h0 = torch.randn(M, D, generator=g, device="cuda").bfloat16()
+    bias = torch.randn(G, D, generator=g, device="cuda")
+    q, s = torch.zeros(M, D, dtype=torch.uint8, device="cuda"), torch.zeros(M, D // 128, device="cuda")
+    h, total = torch.zeros_like(h0), torch.zeros(M, D, device="cuda")
+
+    def steps(pause):
+        st = stream()
+        for i in range(6):
+            tb.check(tb.lib.tsfm_kernel_quantize_e4m3(ptr(h), CODE[h.dtype], M, D, D, 1, ptr(q), D, ptr(s), D // 128, st))
+            pause()
+            tb.check(tb.lib.tsfm_kernel_linear_grouped_e4m3(
+                ptr(q), ptr(s), D // 128, ptr(wq), ptr(ws), D // 128, (D // 128) ** 2, ptr(bias), ptr(h), CODE[h.dtype], 0, 1,
+                ptr(off), G, M, D, D, D, D, D * D, D, st))
+            pause()
+            tb.check(tb.lib.tsfm_kernel_linear_grouped(
+                ptr(h), CODE[h.dtype], ptr(w16), CODE[w16.dtype], None, ptr(total), CODE[total.dtype], 1, 0, ptr(off), G, M, D,
+                D, D, D, D * D, D, st))
+            pause()
+            tb.check(tb.lib.tsfm_kernel_linear_e4m3(ptr(q), ptr(s), D // 128, ptr(wq), ptr(ws), D // 128, None, ptr(h),
+                                                    CODE[h.dtype], 0, 0, M, D, D, D, D, D, st))
+            pause()
+
+    def run(how):
+        h.copy_(h0)
+        total.zero_()
+        how()
+        torch.cuda.synchronize()
+        return h.clone(), total.clone(), q.clone(), s.clone()
+
+    want = run(lambda: steps(torch.cuda.synchronize))
+    assert torch.isfinite(want[1]).all() and want[1].abs().max() > 0
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        steps(lambda: None)
+    for _ in range(10):
+        for got in (run(lambda: steps(lambda: None)), run(graph.replay)):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -268,6 +268,27 @@ Status launch_convert(const float *src, void *dst, int64_t n, int mode, cudaStre
 
 int num_sms();
 
+// A launch whose kernel may become resident before the kernels ahead of it on the stream have completed
+// (it waits for them itself: dep_wait), with `cluster` CTAs a cluster.
+struct DepLaunch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    DepLaunch(dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, int cluster = 1) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)cluster;
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = cluster > 1 ? 2 : 1;
+    }
+};
+
 // Block-scaled E4M3 operands (quantize.cu): q = e4m3(x / s), one scale s per block of block_rows
 // (1 or 128) x 128 elements, s the smallest power of two with max|x| / s <= 448 (at least 2^-126);
 // s and q are NaN for a block that holds an infinity or a NaN. x_dtype E_F32X, E_F16 or E_BF16.

@@ -47,6 +47,9 @@
 // groups' row counts into shared memory before the roles start (32 groups a step). Offsets are
 // clamped to [0, M] and to be nondecreasing, so no content of theirs reaches outside x and y.
 // Every element is summed over K in a fixed order: no atomics, results do not depend on timing.
+// The kernels are launched as dependent ones (dep_wait): in a row of calls the set-up runs under the tail
+// of the call before. us per call, before / with it: one row (N 2304 K 768) 5.5 / 4.7, 77 rows (N 1000
+// K 1032) 7.6 / 6.6, 5000 rows in 8 groups (N 672 K 768) 15.0 / 14.3; large products the same.
 #include "kernels.h"
 #include "ptx.cuh"
 
@@ -118,7 +121,7 @@ __device__ __forceinline__ float silu_fast(float u) { return __fdividef(u, 1.0f 
 // Bias of four consecutive columns of group e (zero past N).
 __device__ __forceinline__ void bias_quad(const BlkArgs &a, int e, int64_t col, float (&b)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = a.bias && col + j < a.N ? __ldg(a.bias + e * a.N + col + j) : 0.0f;
+    for (int j = 0; j < 4; ++j) b[j] = a.bias && col + j < a.N ? a.bias[e * a.N + col + j] : 0.0f;
 }
 
 // y of four consecutive columns of one row (the last columns of a row: fewer): adds to it or not,
@@ -181,8 +184,7 @@ __device__ __forceinline__ void store_sectors(void *o, const float (&v)[32]) {
 
 // The groups' rows and tiles of TILE_M rows, by one warp: group e has rows [g_row[e], g_row[e + 1]) and
 // row tiles [g_tile[e], g_tile[e + 1]). No offsets: one group of M rows.
-// `first` and `o` (a lane's first offset) are loaded before, so that they are on their way while the
-// barriers are initialised. All that runs before the first load of an operand runs once per launch, from
+// `first` and `o` are offsets[0] and a lane's first offset. All that runs before the first load of an operand runs once per launch, from
 // instructions that no cache of the SM holds yet: about 30 cycles each, so loops stay rolled (unrolled,
 // the two scans took 2.5 us) and divisions are by reciprocals from the host.
 template <int TILE_M>
@@ -224,7 +226,7 @@ __device__ __forceinline__ void scan_groups(const BlkArgs &a, int lane, int firs
         }
         end = __shfl_sync(0xffffffffu, o, 31);
         tiles += __shfl_sync(0xffffffffu, t, 31);
-        o = e + 32 < a.groups ? __ldg(a.offsets + e + 33) : 0;
+        o = e + 32 < a.groups ? a.offsets[e + 33] : 0;
     }
 }
 
@@ -300,17 +302,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
         if (lane == 0) *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 0) {
-        const int first = a.offsets ? __ldg(a.offsets) : 0;
-        const int o = a.offsets && lane < a.groups ? __ldg(a.offsets + lane + 1) : 0;
-        if (lane == 0) {
-            tma_prefetch_desc(&tmA);
-            tma_prefetch_desc(&tmB);
-        }
-        scan_groups<C::TILE_M>(a, lane, first, o, g_row, g_tile);
-    }
     if (warp == 1) {
-        __syncwarp();
         if constexpr (PAIR) {
             tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
             tmem_relinquish_pair();
@@ -319,9 +311,20 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
             tmem_relinquish();
         }
     }
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+    }
+    dep_wait();
+    if (warp == 0) {
+        const int first = a.offsets ? *a.offsets : 0;
+        const int o = a.offsets && lane < a.groups ? a.offsets[lane + 1] : 0;
+        scan_groups<C::TILE_M>(a, lane, first, o, g_row, g_tile);
+    }
     tc_fence_before();
     __syncthreads();
     if constexpr (PAIR) cluster_sync_all();
+    dep_release();  // (not before this CTA holds its tensor memory)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -597,7 +600,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
         // address for each of the 128 columns leaves no registers for the sums).
         auto lane_bias = [&](const Tile &tl, int c) {
             const int64_t col = (int64_t)ycol(tl, c) + lane;
-            return col < a.N ? __ldg(a.bias + tl.e * a.N + col) : 0.0f;
+            return col < a.N ? a.bias[tl.e * a.N + col] : 0.0f;
         };
         const uint32_t scales = smem_u32(smem) + C::SCALE_OFF;
         for (int t = unit; t < tiles && ok; t += units) {
@@ -874,9 +877,9 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
 // and the 16 of u) by 32 rows of x in turn. Tiles of fewer units, to share the last round evenly, were
 // slower: what an SM receives is its share of the bytes under way, and 200 KB a CTA keep HBM busy through
 // a round that not all SMs have. Loads start before the block has met.
-// Bound by W's bytes and the start. 32 rows over 24 of 32 groups, N 2048, K 1024: E4M3 13.4 us for 51 MB
-// (3.8 TB/s; the first load is issued after 2.2 us, the last has landed after 11 to 12.3), BF16 21.9 us
-// for 101 MB (4.6 TB/s); 128-wide tiles take 19.6 and 23.3.
+// Bound by W's bytes and the start. 32 rows over 24 of 32 groups, N 2048, K 1024: E4M3 12.6 us for 51 MB
+// (4.0 TB/s; the first load is issued after 2.2 us, the last has landed after 11 to 12.3), BF16 21.0 us
+// for 101 MB (4.8 TB/s); 128-wide tiles take 19.6 and 23.3.
 //   warp 0  offsets, TMA producer        warp 1  tensor memory, MMA issue
 //   warp 3  E4M3: scales                 warps 4..7  epilogue, one unit each
 template <int KIND>
@@ -945,8 +948,6 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
     };
 
     if (warp == 0) {
-        const int first = a.offsets ? __ldg(a.offsets) : 0;
-        const int o = a.offsets && lane < a.groups ? __ldg(a.offsets + lane + 1) : 0;
         if (lane == 0) {
             tma_prefetch_desc(&tmX);
             tma_prefetch_desc(glu ? &tmW : &tmW4);
@@ -955,6 +956,9 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
         for (uint64_t *b = full + lane; b <= drain; b += 32)
             mbar_init(b, (b >= pempty && b < sfull) || (b >= sempty && b < drain) ? 4 : b >= sfull && b < sempty ? 32 : 1);
         fence_barrier_init();
+        dep_wait();
+        const int first = a.offsets ? *a.offsets : 0;
+        const int o = a.offsets && lane < a.groups ? a.offsets[lane + 1] : 0;
         scan_groups<C::ROWS>(a, lane, first, o, g_row, g_tile);
         __syncwarp();
         // The first use of each stage waits for nothing and comes before the block has met.
@@ -1011,9 +1015,11 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
             tmem_relinquish();
             tc_fence_before();
         }
+        dep_wait();
         __syncthreads();
         tc_fence_after();
     }
+    dep_release();  // (not before this CTA holds its tensor memory)
     const uint32_t tmem_base = warp == 0 ? 0u : *tmem_slot;
 
     if (warp == 1) {
@@ -1111,7 +1117,7 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
             const bool mine = unit < tl.cnt;
             const int col = glu ? (tl.n0 + unit) * 16 + (lane & 15) : (tl.n0 + unit) * 32 + lane;
             const bool out = mine && col < a.ycols && (!glu || lane < 16);
-            const float bias = out && a.bias ? __ldg(a.bias + tl.e * a.N + col) : 0.0f;
+            const float bias = out && a.bias ? a.bias[tl.e * a.N + col] : 0.0f;
             float v[32];
             auto tbase = [&]() { return tmem_base + ((uint32_t)(unit * 32) << 16) + (uint32_t)(buf * C::ACC_COLS); };
             if constexpr (F8) {
@@ -1279,8 +1285,8 @@ Status launch_few(const LinearBlocksCall &c, cudaStream_t stream) {
     TSFM_TRY(ensure_smem_attr(reinterpret_cast<const void *>(&linear_few_rows_kernel<KIND>), smem));
     const int64_t most = most_row_tiles(c, C::ROWS) * a.n_tiles;
     if (most > INT32_MAX / 16) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: too many tiles");
-    linear_few_rows_kernel<KIND><<<(unsigned)std::min<int64_t>(most, num_sms()), C::THREADS, smem, stream>>>(tx, tw, tw4, a);
-    const cudaError_t e = cudaGetLastError();
+    DepLaunch l((unsigned)std::min<int64_t>(most, num_sms()), C::THREADS, smem, stream);
+    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, linear_few_rows_kernel<KIND>, tx, tw, tw4, a);
     return e == cudaSuccess ? Status::ok() : Status::cuda(e, "linear (few rows): launch");
 }
 
@@ -1311,19 +1317,9 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     const int64_t most = most_row_tiles(c, C::TILE_M) * a.n_tiles;
     if (most > INT32_MAX / 16) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: too many tiles");
     const int cta = PAIR ? 2 : split;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(split > 1 ? most * split : cta * std::min<int64_t>(most, num_sms() / cta)));
-    cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cta;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cta > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_blocks_kernel<KIND, BN>, ta, tb, ty, a);
+    DepLaunch l((unsigned)(split > 1 ? most * split : cta * std::min<int64_t>(most, num_sms() / cta)), C::THREADS, smem, stream,
+                cta);
+    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, linear_blocks_kernel<KIND, BN>, ta, tb, ty, a);
     if (e != cudaSuccess) return Status::cuda(e, "linear (blocks): launch");
     return Status::ok();
 }

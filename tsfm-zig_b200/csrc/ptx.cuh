@@ -225,8 +225,15 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// ---- TMA ------------------------------------------------------------------------------------
+// Programmatic dependent launch. A kernel launched that way may become resident while the kernels before
+// it on the stream still run: it sets itself up, and touches no data that another kernel may write or
+// read before dep_wait has returned (every kernel before has completed and its writes are visible).
+// dep_release lets the next such kernel become resident in turn. Every CTA of a kernel waits, so that
+// its completion implies that of all before it.
+__device__ __forceinline__ void dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void dep_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// ---- TMA ------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }

@@ -148,6 +148,8 @@ template <int DT, int U>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeCall c, int64_t blocks, uint32_t per_row, bool vx,
                                                             bool vq) {
     constexpr int esz = DT == E_F32X ? 4 : 2;
+    dep_wait();
+    dep_release();
     const int lane = threadIdx.x & 7, at = threadIdx.x >> 3;
     const int64_t first = (int64_t)blockIdx.x * (32 * U);
     const int64_t r0 = first / per_row;
@@ -190,6 +192,8 @@ template <int DT>
 __global__ void __launch_bounds__(256) quantize_tiles_kernel(QuantizeCall c, bool vx, bool vq) {
     __shared__ uint32_t warp_max[8];
     constexpr int esz = DT == E_F32X ? 4 : 2;
+    dep_wait();
+    dep_release();
     const int lane = threadIdx.x & 7, r0 = threadIdx.x >> 3;
     const int col = (int)blockIdx.x * 128 + lane * 16, n = (int)c.cols - col;
     for (int64_t br = blockIdx.y; br * 128 < c.rows; br += gridDim.y) {
@@ -225,18 +229,20 @@ Status launch_dt(const QuantizeCall &c, cudaStream_t stream) {
     const bool vx = (reinterpret_cast<uintptr_t>(c.x) & 15) == 0 && (c.ldx * esz) % 16 == 0;
     const bool vq = (reinterpret_cast<uintptr_t>(c.q) & 15) == 0 && c.ldq % 16 == 0;
     const int64_t per_row = (c.cols + 127) / 128;
+    cudaError_t e;
     if (c.block_rows == 1) {
         const int64_t blocks = c.rows * per_row;
         constexpr int U = DT == E_F32X ? 1 : 2;  // 64 bytes a thread in flight
         const int64_t ctas = (blocks + 32 * U - 1) / (32 * U);
         if (ctas > INT32_MAX) return Status::fail(TSFM_ERR_UNSUPPORTED, "quantize: too many blocks");
-        quantize_rows_kernel<DT, U><<<(unsigned)ctas, 256, 0, stream>>>(c, blocks, (uint32_t)per_row, vx, vq);
+        DepLaunch l((unsigned)ctas, 256, 0, stream);
+        e = cudaLaunchKernelEx(&l.cfg, quantize_rows_kernel<DT, U>, c, blocks, (uint32_t)per_row, vx, vq);
     } else {
         const int64_t tiles = (c.rows + 127) / 128;
         const dim3 grid((unsigned)per_row, (unsigned)std::min<int64_t>(tiles, 65535));
-        quantize_tiles_kernel<DT><<<grid, 256, 0, stream>>>(c, vx, vq);
+        DepLaunch l(grid, 256, 0, stream);
+        e = cudaLaunchKernelEx(&l.cfg, quantize_tiles_kernel<DT>, c, vx, vq);
     }
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? Status::ok() : Status::cuda(e, "quantize: launch");
 }
 
