@@ -535,6 +535,45 @@ def test_feed_forward_chain():
     assert ((xv - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * xs.double().repeat_interleave(128, 1)).all()
 
 
+@pytest.mark.parametrize("M", [5, 60, 400, 3000])
+def test_gated_nan_stays_in_its_column(M):
+    # one weight of g and one of u are NaN: their output columns are, the ones beside them not; and u far
+    # below zero, where the gate's exponential leaves FP32
+    N, K = 1024, 256
+    c = Case(M, N, K, "e4m3", seed=11)
+    k = 0.5 / float(c.ref.std())
+    c.xs *= k
+    c.ref, c.tol = c.ref * k, 1.1 * c.tol * k
+    c.check(torch.bfloat16, act=3)
+    y0 = torch.zeros(M, N // 2, device="cuda", dtype=torch.bfloat16)
+    y1 = torch.zeros_like(y0)
+    tb.check(c.call(y0, act=3))
+    torch.cuda.synchronize()
+    c.w[0, 20, 3] = float("nan")            # g of column 20
+    c.w[0, 256 + 128 + 71, 9] = float("nan")  # u of column 128 + 71
+    tb.check(c.call(y1, act=3))
+    torch.cuda.synchronize()
+    hit = torch.zeros(N // 2, dtype=torch.bool, device="cuda")
+    hit[[20, 199]] = True
+    assert torch.isnan(y1[:, hit]).all() and torch.equal(y1[:, ~hit], y0[:, ~hit])
+    # u = -3e4 in column 5 (one weight row of -448, an x of 448 in its place): g silu(u) is 0 to within
+    # 3e4 * 2^-60 of |g|
+    d = Case(M, N, K, "e4m3", seed=12)
+    d.x.zero_()
+    d.x[:, 0] = 448.0
+    d.w.zero_()
+    d.w[0, :128, 0] = 1.0
+    d.w[0, 128:256, 0] = 1.0
+    d.w[0, 128 + 5, 0] = -448.0
+    d.xs.fill_(1 / 448.0)
+    d.ws.fill_(1.0)
+    d.ws[0, 1, 0] = 70.0  # u = 70, and -31360 in column 5; g = 1
+    tb.check(d.call(y1, act=3))
+    torch.cuda.synchronize()
+    assert (y1[:, :5] == 70.0).all() and (y1[:, 6:128] == 70.0).all() and (y1[:, 128:] == 0).all()
+    assert (y1[:, 5].float().abs() <= 31360 * 2.0 ** -60).all()
+
+
 @pytest.mark.parametrize("M", [5, 300, 3000])
 def test_back_to_back_calls_see_their_predecessors(M):
     # Calls that read what the call before wrote and overwrite what it read, without a pause between

@@ -599,6 +599,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 
+// 1 / x there (within one unit in the last place; x past 2^126 gives 0).
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Round an FP32 value to TF32 (round to nearest, ties away), as the tensor cores consume it.
 __device__ __forceinline__ float to_tf32(float x) {
     uint32_t r;
