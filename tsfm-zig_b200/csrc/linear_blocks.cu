@@ -23,25 +23,26 @@
 //               through 4 KB of shared memory a warp). E4M3 on 256 columns with a 16-bit y: through
 //               boxes of 64 columns to TMA stores, so that the tile leaves while the next is summed.
 // E4M3 on 256 columns: each warpgroup of the epilogue has accumulators of its own (two of 128
-// columns), filled by MMAs of its half of the columns, so that handing one back and forth (MMA 256
-// cycles, commit and waits 300, loads 350) takes less than the 1024 cycles that the tensor cores
-// need for two blocks of K.
+// columns), filled by MMAs of its half of the columns, so that one half's sums are
+// loaded while the other half's are made.
 // Rows of a group that end inside a tile: the tile's other rows hold whatever follows in x (or the
 // stage's old bytes), are computed and not stored.
 //
 // What bounds it (B200, 148 SMs, random operands):
-//   16 bits, 256 x 256  the tensor cores: their pipe is active 80 % of the time at M 16384, N 4096,
-//                       K 1024 in 16 groups, 1491 TFLOP/s at M 32768 in 32 groups (184 us).
-//   E4M3, 256 x 256     the epilogue's passes over the accumulators: loads and MMAs alone take 374 ns a
-//                       block of K (3135 TFLOP/s), with the passes 470 ns (K 4096: 278 us for M 75776,
-//                       N 1024, 2282 TFLOP/s); at K 768 a tile's finish is a third (1600 TFLOP/s at
-//                       M 73856, N 2304, 161 us; tensor pipe 38 %). A pass is a chain of waits, tensor-
-//                       memory loads and packed FMAs on two warps per scheduler: 128 sums and 64 loaded
-//                       values a thread leave no room for more warps.
+//   16 bits, 256 x 256  the tensor cores: their pipe is active 82 % of the time at M 16384, N 4096,
+//                       K 1024 in 16 groups, 1530 TFLOP/s at M 32768 in 32 groups (179 us); in a row of
+//                       calls the power limit (the same 262,000 cycles at 1.1 to 1.3 GHz, 200 to 235 us).
+//   E4M3, 256 x 256     handing accumulators over: a block of K takes 850 cycles (K 4096: 278 us for
+//                       M 75776, N 1024, 2282 TFLOP/s) where the tensor cores need 512. With nothing
+//                       added to the sums it takes 705, with one load a pass 693: two accumulators a half
+//                       and 1390 cycles for one's round (MMA, commit, wait, loads, hand-back). At K 768 a
+//                       tile's finish is 1500 of 7200 cycles (1636 TFLOP/s at M 73856, N 2304, 160 us).
+//                       128 sums and 64 loaded values a thread leave no room for more warps, 512
+//                       columns of tensor memory none for more accumulators.
 //   few rows            the start and W's bytes; groups of few rows have a kernel of their own below.
 // Tried and slower: 128 x 256 tiles on one SM (their loads alone 526 ns a block of K), there also 16
-// epilogue warps of 64 columns (registers spill; 401 ns against 377 for 8 warps), test_wait in place of
-// try_wait (2 %).
+// epilogue warps of 64 columns (registers spill; 401 ns against 377 for 8 warps), one MMA over all 256
+// columns in place of two halves (875 cycles a block), test_wait in place of try_wait (2 %).
 //
 // Groups: the offsets are device memory, so the tile list is made on the device: warp 0 scans the
 // groups' row counts into shared memory before the roles start (32 groups a step). Offsets are
