@@ -1337,12 +1337,12 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
 }
 
 // The tile width by the time that its waves of tiles take: a start, and per wave a part per stage of
-// K and one per tile (units of 100 ns, fitted to M 1-4096, N 768-4096, K 768-4096; the fit need only
+// K and one per tile (units of 100 ns, fitted to M 256-4096, N 768-4096, K 768-4096; the fit need only
 // rank the widths). Groups: each is taken to end in the middle of a tile. Measured, E4M3, us for widths
 // 64 / 128 / 256:
-//   M 512  N 2304 K 768   6.6 /  7.0 / 10.8      M 2048 N 4096 K 1024  24.1 / 19.7 / 18.6
-//   M 1024 N 2304 K 768   8.9 /  7.3 / 11.2      M 4096 N 4096 K 1024  42.8 / 30.5 / 29.2
-//   M 2048 N 1024 K 4096 22.6 / 15.6 / 22.8      M 4096 N 1024 K 4096  40.4 / 27.4 / 24.3
+//   M 512  N 2304 K 768   6.0 /  6.6 / 10.0      M 4096 N 2304 K 768   26.9 / 18.1 / 15.4
+//   M 1024 N 2304 K 768   8.8 /  6.8 / 10.1      M 2048 N 4096 K 1024  26.9 / 20.3 / 17.1
+//   M 2048 N 1024 K 4096 21.9 / 15.0 / 21.5      M 4096 N 1024 K 4096  39.7 / 27.0 / 23.2
 template <int KIND>
 int tile_width(const LinearBlocksCall &c) {
     struct Cost {
@@ -1351,9 +1351,9 @@ int tile_width(const LinearBlocksCall &c) {
     };
     const int sms = num_sms();
     const bool f8 = KIND == E_U8;
-    const Cost costs[3] = {{64, 128, sms, 0, f8 ? 2.6 : 2.2, f8 ? 6.0 : 3.0},
-                           {128, 128, sms, 0, f8 ? 3.0 : 2.8, f8 ? 8.0 : 3.0},
-                           {256, 256, sms / 2, f8 ? 30.0 : 35.0, f8 ? 4.4 : 3.6, f8 ? 12.0 : 5.0}};
+    const Cost costs[3] = {{64, 128, sms, 0, f8 ? 2.3 : 2.2, f8 ? 16.4 : 3.0},
+                           {128, 128, sms, 0, f8 ? 3.3 : 2.8, f8 ? 18.7 : 3.0},
+                           {256, 256, sms / 2, f8 ? 32.0 : 35.0, f8 ? 4.8 : 3.6, f8 ? 20.0 : 5.0}};
     const int64_t stages = (c.K + (f8 ? 127 : 63)) / (f8 ? 128 : 64);
     int best = 128;
     double least = 1e300;
