@@ -301,7 +301,9 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
 
 /* 8-bit operands with a scale per block, and products grouped by expert. Device pointers on the
  * current device; all return after enqueueing on `stream`, allocate nothing on it and can be
- * captured. None has a counterpart in the reference (it has one FP32 product per layer).
+ * captured. None has a counterpart in the reference (it has one FP32 product per layer). They are
+ * launched as programmatic dependents: a kernel may become resident early, but reads and writes data
+ * only after all work ahead of it on the stream has completed.
  *
  * tsfm_kernel_quantize_e4m3: x [rows, cols] (F32, F16 or BF16, row stride ldx elements) to E4M3
  *   codes q [rows, cols] (bytes, row stride ldq) and one FP32 scale per block of block_rows x 128
