@@ -1315,7 +1315,9 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     const int ysz = c.y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
     a.vec = reinterpret_cast<uintptr_t>(c.y) % (4 * ysz) == 0 && c.ldy % 4 == 0;
     a.vec32 = reinterpret_cast<uintptr_t>(c.y) % 32 == 0 && (c.ldy * ysz) % 32 == 0;
-    a.y_tma = C::TMA_Y && ysz == 2 && !c.accumulate && reinterpret_cast<uintptr_t>(c.y) % 16 == 0 && c.ldy % 8 == 0;
+    // A TMA store clips a row to whole 16 bytes: with other numbers of columns it would write the padding.
+    a.y_tma = C::TMA_Y && ysz == 2 && !c.accumulate && reinterpret_cast<uintptr_t>(c.y) % 16 == 0 && c.ldy % 8 == 0 &&
+              a.ycols % 8 == 0;
     ty = ta;
     if (a.y_tma) {
         const int64_t d[2] = {a.ycols, c.M}, st[2] = {1, c.ldy};

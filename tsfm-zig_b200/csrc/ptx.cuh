@@ -281,7 +281,8 @@ __device__ __forceinline__ void tma_load_5d_pair(void *smem_dst, const CUtensorM
 }
 
 // 2-D tiled store of a shared-memory box to global memory at (c0 = innermost, c1), tracked by this
-// thread's bulk-async groups. Rows and columns outside the tensor are not written.
+// thread's bulk-async groups. Rows outside the tensor are not written, nor columns outside a tensor
+// whose rows are a multiple of 16 bytes (of others, the rest of the last 16 bytes is written too).
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *smem_src, int32_t c0, int32_t c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                      reinterpret_cast<uint64_t>(map)),
