@@ -555,3 +555,27 @@ def test_linear_weight_term_only(M, N, K):
     ref = xh @ w.double().T
     mag = xh.abs() @ w.double().abs().T
     assert ((y.double() - ref).abs() <= 2.0 ** -12 * mag + 1e-6).all()
+
+
+@pytest.mark.parametrize("M", [300, 4100])
+@pytest.mark.parametrize("N,pad", [(70, 2), (131, 5), (1001, 7), (1300, 4), (602, 30)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "tf32"])
+def test_linear_leaves_the_padding_of_rows(M, N, pad, dtype):
+    # rows of y longer than N whose stride suits TMA stores, with an N that does not fill its last 16 bytes:
+    # stored, activated and accumulated, the columns past N keep what they held. Operands of small whole
+    # numbers: every sum is exact in FP32 (and, below 256, in 16 bits).
+    K = 64
+    g = torch.Generator(device="cpu").manual_seed(M + N)
+    t = TORCH16.get(dtype, torch.float32)
+    x = torch.randint(-1, 2, (M, K), generator=g).to(dev(), t)
+    w = torch.randint(-2, 3, (N, K), generator=g).to(dev(), t)
+    bias = torch.randint(-9, 10, (N,), generator=g).to(dev(), torch.float32)
+    ref = x.double() @ w.double().T
+    for out_mode, act, b in ((1, 0, bias), (1, 1, None), (2, 0, None), (2, 1, bias)) + (() if dtype == "tf32" else ((0, 0, None), (0, 1, bias))):
+        y = torch.full((M, N + pad), -5.0, device=dev(), dtype=t if out_mode == 0 else torch.float32)
+        linear(x, w, b, y, out_mode, act, M, N, K)
+        want = ref + (0 if b is None else b.double()) - (5 if out_mode == 2 else 0)
+        if act:
+            want = want.clamp(min=0)
+        assert torch.equal(y[:, :N].double(), want), (out_mode, act)
+        assert (y[:, N:] == -5.0).all(), (out_mode, act)

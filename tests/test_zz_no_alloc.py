@@ -116,3 +116,17 @@ def test_noalloc_rejects_products_beyond_its_scratch():
     st = noalloc(A, B, C, 1.0, torch.cuda.current_stream().cuda_stream)
     assert tb.STATUS_NAMES[st] == "INVALID_ARGUMENT"
     assert "scratch limit" in tb.last_error()
+
+
+@pytest.mark.parametrize("m,n,k,ldc", [(61, 70, 40, 72), (300, 131, 64, 136), (40, 3, 8, 4)])
+def test_noalloc_keeps_padding_of_aligned_rows(m, n, k, ldc):
+    # rows of C of whole 16 bytes, an n that does not fill the last ones
+    g = torch.Generator().manual_seed(m + n)
+    A = torch.randint(-2, 3, (m, k), generator=g).float().cuda()
+    B = torch.randint(-2, 3, (n, k), generator=g).float().cuda()
+    flat = torch.full((m * ldc,), -5.0, device="cuda")
+    st = tb.lib.tsfm_sgemm_nt_noalloc(m, n, k, 1.0, A.data_ptr(), k, B.data_ptr(), k, flat.data_ptr(), ldc,
+                                      torch.cuda.current_stream().cuda_stream)
+    assert st == 0, tb.last_error()
+    C = flat.view(m, ldc)
+    assert torch.equal(C[:, :n].double(), A.double() @ B.double().T) and (C[:, n:] == -5.0).all()

@@ -72,6 +72,7 @@ struct LinearCall {
     int64_t M = 0, N = 0, K = 0, ldx = 0, ldw = 0;
     void *y = nullptr;
     int64_t ldy = 0;
+    bool y_pad_free = false;  // the rest of a row's last 16 bytes, within ldy, may be written too
     int out_mode = OUT_BF16;  // OutMode; OUT_F32_ACC: y += result
     const float *bias = nullptr;
     // 0 none, 1 relu, 2 silu, ACT_GLU: gated pairs. With ACT_GLU the weight's rows come in 256-row

@@ -960,14 +960,16 @@ Status launch_t(const LinearCall &c, cudaStream_t stream) {
     e.ldnx8 = c.ld_nx8;
     e.nx8_half = c.N;
     // TMA epilogue unless rows are remapped or an activation follows the accumulation; the
-    // output base and row stride must suit a tensor map (16-byte alignment).
+    // output base and row stride must suit a tensor map (16-byte alignment), and its columns fill whole
+    // 16 bytes (a TMA store clips a row to those) unless the caller lets the padding be written.
     const bool f32_out = c.out_mode == OUT_F32 || c.out_mode == OUT_F32_ACC || c.out_mode == OUT_TF32;
     e.tma_mode = 0;
     CUtensorMap ty = tb;
     if (c.rm_g <= 0 && !(c.out_mode == OUT_F32_ACC && c.act != 0)) {
         const int ydt = f32_out ? E_F32 : c.out_mode == OUT_F16 ? E_F16 : E_BF16;
         const int64_t ycols = c.act == ACT_GLU ? c.N / 2 : c.N;
-        if (make_tmap(&ty, c.y, ydt, ycols, c.M, c.ldy, f32_out ? 32 : 64, 32).code == 0)
+        if ((ycols * (f32_out ? 4 : 2) % 16 == 0 || c.y_pad_free) &&
+            make_tmap(&ty, c.y, ydt, ycols, c.M, c.ldy, f32_out ? 32 : 64, 32).code == 0)
             e.tma_mode = c.out_mode == OUT_F32_ACC ? 2 : 1;
     }
     if constexpr (NORM) {

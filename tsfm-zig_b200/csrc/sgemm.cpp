@@ -113,6 +113,7 @@ Status sgemm_impl(int m, int n, int k, float alpha, const float *A, int lda, con
     lc.ldw = kp;
     lc.y = x->c.p;
     lc.ldy = np;
+    lc.y_pad_free = true;  // rows of this call's own buffer
     lc.err = static_cast<int *>(x->err.p);
     lc.x = alo;
     lc.w = bhi;
