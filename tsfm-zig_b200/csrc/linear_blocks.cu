@@ -121,13 +121,22 @@ struct BlkArgs {
 __device__ __forceinline__ float silu_fast(float u) { return u * rcp_approx(1.0f + ex2_approx(-1.44269504f * u)); }
 
 // g silu(u) of two columns with one reciprocal, 1 / a = b / (a b): the special-function unit, 16 results a
-// clock, bounds the finish of a gated tile. Each factor is held to 2^60, so that the product stays in
-// range and a NaN in its own column; that bends silu below u = -41 only, where it is under 4e-17.
+// clock, bounds the finish of a gated tile. Each exponential is held to 2^60, so that the product of the
+// factors stays in range and a NaN in its own column; below kGateFar that gives u 2^-60 in place of silu
+// (held to -1: g times it stays finite), which gate_far makes up for.
+constexpr float kGateFar = -41.588831f;  // e^-u = 2^60
 __device__ __forceinline__ float2 gate_pair(float2 g, float2 u) {
     const float a = 1.0f + fminf(ex2_approx(-1.44269504f * u.x), 0x1p60f);
     const float b = 1.0f + fminf(ex2_approx(-1.44269504f * u.y), 0x1p60f);
     const float r = rcp_approx(a * b);
-    return make_float2(g.x * (u.x * (b * r)), g.y * (u.y * (a * r)));
+    return make_float2(g.x * max_nan(u.x * (b * r), -1.0f), g.y * max_nan(u.y * (a * r), -1.0f));
+}
+
+// gate_pair's result f of a column, times 2^60 e^u where u is below kGateFar: to zero, as silu goes, and to
+// NaN at -infinity (-infinity / infinity).
+__device__ __forceinline__ float gate_far(float f, float u) {
+    if (!(u < kGateFar)) return f;
+    return f * (ex2_approx(fmaf(1.44269504f, u, 60.0f)) + (u - u));
 }
 
 // Bias of four consecutive columns of group e (zero past N).
@@ -725,10 +734,24 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     // next one is summed. One branch per step of all chunks: with branches per chunk and word
                     // this part took 2100 cycles a tile.
                     if (glu) {
+                        float least = 0.0f;
 #pragma unroll
                         for (int c = 0; c < CPH; ++c)
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) acc[c][j] = gate_pair(acc[c][j], acc[c + CPH][j]);
+                            for (int j = 0; j < 16; ++j) {
+                                const float2 u = acc[c + CPH][j];
+                                acc[c][j] = gate_pair(acc[c][j], u);
+                                least = fminf(fminf(least, u.x), u.y);
+                            }
+                        if (least < kGateFar) {
+#pragma unroll
+                            for (int c = 0; c < CPH; ++c)
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    acc[c][j].x = gate_far(acc[c][j].x, acc[c + CPH][j].x);
+                                    acc[c][j].y = gate_far(acc[c][j].y, acc[c + CPH][j].y);
+                                }
+                        }
                     } else if (a.bias) {
 #pragma unroll
                         for (int c = 0; c < CH; ++c) {
@@ -780,10 +803,16 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     if (glu) {
                         float u[32];
                         chunk((c + CPH) % CH, u);
+                        float least = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             const float2 f = gate_pair(make_float2(v[j], v[j + 1]), make_float2(u[j], u[j + 1]));
                             v[j] = f.x, v[j + 1] = f.y;
+                            least = fminf(fminf(least, u[j]), u[j + 1]);
+                        }
+                        if (least < kGateFar) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = gate_far(v[j], u[j]);
                         }
                     } else if (a.bias) {
                         const float b = lane_bias(tl, c);

@@ -600,6 +600,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 
+// The larger of two, NaN if either is (fmaxf passes over a NaN).
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
 // 1 / x there (within one unit in the last place; x past 2^126 gives 0).
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
