@@ -76,6 +76,60 @@ def test_gate_far_below_zero(form, kind):
                 assert not bad.any(), (su, sg, dtype, pad, int(bad.sum()), out[bad][:4].tolist(), ref[bad][:4].tolist())
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_whose_product_leaves_fp32(form):
+    # y = sum_b xs ws S_b for scales of which the product of two is past FP32 (blocks 1 of K: 2^140) or below
+    # its normal numbers (blocks 2: 2^-140, 2^-150): rows of x whose codes are zero in the blocks of the
+    # first kind keep the others' sum; rows of one subnormal code there reach 2^122; rows that have codes in
+    # the blocks of the second kind alone reach 2^-115. Tolerance: that of Case, with one more rounding.
+    M, N, _, counts = FORMS[form]
+    K = 4096 if form == "shared" else 700
+    c = Case(M, N, K, "e4m3", counts=counts, seed=22)
+    kb, G = -(-K // 128), c.groups
+    r = gen(M * 3 + N)
+    blk = torch.arange(K, device="cuda") // 128 % 4
+    row = torch.arange(M, device="cuda") % 3
+    cx = c.x[:, :K].view(torch.uint8)
+    cw = c.w[:, :, :K].view(torch.uint8)
+    cw[:, :, blk == 1] = torch.randint(1, 4, (G, N, int((blk == 1).sum())), generator=r, device="cuda", dtype=torch.uint8)
+    cx[:, blk == 1] = 0
+    tiny = torch.zeros(M, K, dtype=torch.bool, device="cuda")
+    tiny[row == 1, 130] = True
+    cx[tiny] = 1
+    cx[(row == 2)[:, None] & (blk != 2)[None]] = 0
+    xs = c.xs[:, :kb]
+    ws = c.ws[:, :, :kb]
+    kind = torch.arange(kb, device="cuda") % 4
+    xs.copy_(1 + torch.rand(M, kb, generator=r, device="cuda"))
+    ws.copy_((1 + torch.rand(G, ws.shape[1], kb, generator=r, device="cuda")))
+    ws[:, 0::2] *= -1
+    xs[:, kind == 1] *= 2.0 ** 100
+    ws[:, :, kind == 1] *= 2.0 ** 40
+    xs[0::2, kind == 2] *= 2.0 ** -100
+    xs[1::2, kind == 2] *= 2.0 ** -110
+    ws[:, :, kind == 2] *= 2.0 ** -40
+    xd = c.x[:, :K].double() * xs.double().repeat_interleave(128, 1)[:, :K]
+    unit = (K + 3 * kb + 8) * 2.0 ** -23
+    for e in range(G):
+        lo, hi = (0, M) if counts is None else (int(c.off[e]), int(c.off[e + 1]))
+        wd = c.w[e, :, :K].double() * ws[e].double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+        c.ref[lo:hi] = xd[lo:hi] @ wd.T
+        c.tol[lo:hi] = unit * (xd[lo:hi].abs() @ wd.abs().T)
+    assert c.ref[c.used & (row == 1)].abs().min() > 2.0 ** 110 and c.ref[c.used & (row == 2)].abs().max() < 2.0 ** -110
+    for dtype in (torch.float32, torch.bfloat16):
+        y = torch.full((M, N), 5.0, device="cuda", dtype=dtype)
+        tb.check(c.call(y))
+        torch.cuda.synchronize()
+        out = y.double()
+        # the smallest numbers: every sum of a block rounds once more to a multiple of 2^-149
+        lim = c.tol + torch.finfo(dtype).eps / 2 * (c.ref.abs() + c.tol) + (kb + 1) * 2.0 ** -149
+        if dtype == torch.bfloat16:
+            lim = lim + 2.0 ** -134
+        bad = ~((out - c.ref).abs() <= lim) & c.used[:, None]
+        assert not bad.any(), (dtype, int(bad.sum()), [int((bad[row == i]).sum()) for i in range(3)],
+                               out[bad][:4].tolist(), c.ref[bad][:4].tolist())
+
+
 @pytest.mark.parametrize("M,N,K", [(8000, 1000, 768), (9001, 1001, 392), (7000, 1300, 768)])
 def test_partial_boxes_leave_the_padding(M, N, K):
     # 16-bit outputs of 256 x 256 tiles leave in boxes of 64 columns x 32 rows: the last ones are clipped to

@@ -17,7 +17,8 @@
 //               one per tile (16 bits, two in turn) or one per block of K (E4M3).
 //   warp 2      E4M3, 256 columns: issues the TMA stores of the boxes that the epilogue fills.
 //   warp 3      E4M3: the scales of the tile's rows and columns into a ring of shared memory, four
-//               blocks of K at a time, ahead of the tiles that need them.
+//               blocks of K at a time, ahead of the tiles that need them, marked where a product of two
+//               of them leaves FP32 (the mark costs the 256-wide tiles 2 %; looked for by the epilogue, 4 %).
 //   warps 4..   epilogue: a thread owns a row and 128 (below 256 columns: 64) of its columns, which
 //               are whole 32-byte sectors of y (columns past N, other alignments and sums into y pass
 //               through 4 KB of shared memory a warp). E4M3 on 256 columns with a 16-bit y: through
@@ -66,7 +67,7 @@ constexpr int kMaxGroups = 1024;  // two words of shared memory each
 
 // Blocks of K whose scales share a slot of the ring, and the slots.
 constexpr int kScaleQuad = 4, kScaleSlots = 4;
-constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2) * 4;  // [row][block of K], then [half tile][block of K]
+constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2 + 1) * 4;  // [row][block of K], [half tile][block of K], wide
 
 // KIND: element type of x and W (E_F16, E_BF16, E_U8 = E4M3).
 template <int KIND, int BN>
@@ -138,6 +139,33 @@ __device__ __forceinline__ float gate_far(float f, float u) {
     if (!(u < kGateFar)) return f;
     return f * (ex2_approx(fmaf(1.44269504f, u, 60.0f)) + (u - u));
 }
+
+// A block's scale is the FP32 product s = xs ws, a normal number but for odd data. wide_scale: it is past FP32,
+// or subnormal and not exact. (A row of zeros has the quantiser's least scale, a power of two; and since a
+// block's sum is below 2^25, a scale below 2^-176 gives 0 in any case.)
+__device__ __forceinline__ bool wide_scale(float xs, float ws) {
+    const float s = xs * ws, m = fabsf(s);
+    if (m > 1.0f) return m > 0x1.fffffep127f && fabsf(xs) <= 0x1.fffffep127f && fabsf(ws) <= 0x1.fffffep127f;
+    if (!(m < 0x1p-126f)) return false;
+    const float t = (xs * 0x1p50f) * (ws * 0x1p50f);
+    return fabsf(t) >= 0x1p-76f && s * 0x1p100f != t;
+}
+
+// Such a block's sums are multiplied by a power of two (returned) before they meet s, now xs ws over that
+// power: 2^127 or 2^-100. Sums are multiples of 2^-18, so the first step is exact or leaves FP32 as the result
+// does; s held to FP32's largest number changes none that is not past FP32 itself.
+__device__ __forceinline__ float split_scale(float xs, float ws, float &s) {
+    s = xs * ws;
+    if (!wide_scale(xs, ws)) return 1.0f;
+    if (fabsf(s) > 1.0f) {
+        s = copysignf(fminf(fabsf((xs * 0x1p-64f) * (ws * 0x1p-63f)), 0x1.fffffep127f), s);
+        return 0x1p127f;
+    }
+    s = (xs * 0x1p50f) * (ws * 0x1p50f);
+    return 0x1p-100f;
+}
+
+__device__ __forceinline__ bool ordinary_scales(float least, float most) { return least >= 0x1p-126f && most <= 0x1.fffffep127f; }
 
 // Bias of four consecutive columns of group e (zero past N).
 __device__ __forceinline__ void bias_quad(const BlkArgs &a, int e, int64_t col, float (&b)[4]) {
@@ -317,7 +345,6 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
     if (warp == 2) {
         for (uint64_t *b = full + lane; b <= drain; b += 32)
             mbar_init(b, b >= pempty && b < sfull    ? (PAIR ? 2 : 1) * C::EPI_WARPS / NH  // one arrival per epilogue warp
-                         : b >= sfull && b < sempty  ? 32
                          : b >= sempty && b < bfull  ? C::EPI_WARPS
                                                      : 1);
         if (lane == 0) *abort_flag = 0;
@@ -556,16 +583,53 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
             }
         } else if (F8 && warp == 3) {
             // Scales: slot = xs[128][4] then ws[2][4] (the half tiles' column blocks), by asynchronous
-            // copies; entries past this CTA's last block of K are not read.
-            int slot = 0;
+            // copies; past this CTA's last block of K its scales again. A slot is looked through for wide scales
+            // and handed over once the copies of the next one are under way.
+            int slot = 0, landing = -1;
             uint32_t ph = 0;
             bool ok = true;
+            auto hand_over = [&]() {
+                __syncwarp();
+                const uint32_t d = smem_u32(smem) + C::SCALE_OFF + landing * kScaleSlotBytes;
+                float w0[4], w1[4], x[4];
+                ld_shared_v4(d + 2048, w0);
+                ld_shared_v4(d + 2064, w1);
+                // The smallest and the largest of xs times those of ws (a NaN is passed over).
+                float x_least = 0x1.fffffep127f, x_most = 0.0f, w_least = x_least, w_most = 0.0f;
+                for (int r = lane; r < 128; r += 32) {
+                    ld_shared_v4(d + r * 16, x);
+#pragma unroll
+                    for (int j = 0; j < kScaleQuad; j += 2) {
+                        x_least = fminf(fminf(x_least, fabsf(x[j])), fabsf(x[j + 1]));
+                        x_most = fmaxf(fmaxf(x_most, fabsf(x[j])), fabsf(x[j + 1]));
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kScaleQuad; ++j) {
+                    w_least = fminf(fminf(w_least, fabsf(w0[j])), fabsf(w1[j]));
+                    w_most = fmaxf(fmaxf(w_most, fabsf(w0[j])), fabsf(w1[j]));
+                }
+                bool wide = false;
+                if (!__all_sync(0xffffffffu, ordinary_scales(x_least * w_least, x_most * w_most))) {
+#pragma unroll 1
+                    for (int r = lane; r < 128; r += 32) {
+                        ld_shared_v4(d + r * 16, x);
+#pragma unroll
+                        for (int j = 0; j < kScaleQuad; ++j) wide = wide || wide_scale(x[j], w0[j]) || wide_scale(x[j], w1[j]);
+                    }
+                    wide = __any_sync(0xffffffffu, wide) != 0;
+                }
+                if (lane == 0) {
+                    st_shared_f32(d + 2080, wide ? 1.0f : 0.0f);
+                    mbar_arrive(&sfull[landing]);
+                }
+            };
             for (int t = unit; t < tiles && ok; t += units) {
                 const Tile tl = tile_at(t);
                 const float *xs = a.xs + (int64_t)tl.row0 * a.ld_xs;
                 const int last = tl.row_end - 1 - tl.row0;  // rows past the group's end repeat its last
                 const int nb = min((lane & 4 ? tl.b1 : tl.b0) >> 7, a.ws_blocks - 1);
-                const float *ws = a.ws + tl.e * a.ws_group + (int64_t)nb * a.ld_ws + (lane & 3);
+                const float *ws = a.ws + tl.e * a.ws_group + (int64_t)nb * a.ld_ws;
                 for (int kb = kb0; kb < kb1; kb += kScaleQuad) {
                     ok = wait(&sempty[slot], ph ^ 1u, ERR_SITE_BLOCKS_PRODUCER);
                     if (!ok) break;
@@ -573,10 +637,16 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     const int n = min(kScaleQuad, kb1 - kb);
                     for (int r = lane; r < 128; r += 32) {
                         const float *src = xs + (int64_t)min(r, last) * a.ld_xs + kb;
-                        for (int j = 0; j < n; ++j) cp_async_4(d + r * 16 + j * 4, src + j);
+#pragma unroll
+                        for (int j = 0; j < kScaleQuad; ++j) cp_async_4(d + r * 16 + j * 4, src + min(j, n - 1));
                     }
-                    if (lane < 8 && (lane & 3) < n) cp_async_4(d + 2048 + lane * 4, ws + kb);
-                    cp_async_arrive(&sfull[slot]);
+                    if (lane < 8) cp_async_4(d + 2048 + lane * 4, ws + kb + min(lane & 3, n - 1));
+                    cp_async_commit();
+                    if (landing >= 0) {
+                        cp_async_wait_1();
+                        hand_over();
+                    }
+                    landing = slot;
                     if (++slot == kScaleSlots) {
                         slot = 0;
                         ph ^= 1u;
@@ -584,6 +654,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                 }
             }
             cp_async_wait_all();
+            if (ok && landing >= 0) hand_over();
         }
     } else {
         if constexpr (SPLIT_REGS) regs_inc<232>();
@@ -646,21 +717,53 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     ld_shared_v4(sc + (eg * 32 + lane) * 16, xv);
                     ld_shared_v4(sc + 2048, w0);
                     ld_shared_v4(sc + 2064, w1);
+                    const bool wide = ld_shared_f32(sc + 2080) != 0.0f;
 #pragma unroll
                     for (int j = 0; j < kScaleQuad; ++j) s0[j] = xv[j] * w0[j], s1[j] = xv[j] * w1[j];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sempty[slot]);
-                    if (++slot == kScaleSlots) {
-                        slot = 0;
-                        sph ^= 1u;
-                    }
                     const int n = min(kScaleQuad, kbn - kb);
-#pragma unroll 1
-                    for (int j = 0; j < n; ++j) {
+                    auto used = [&]() {  // the slot's scales
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sempty[slot]);
+                        if (++slot == kScaleSlots) {
+                            slot = 0;
+                            sph ^= 1u;
+                        }
+                    };
+                    auto ready = [&]() {
                         ok = wait_epi(&pfull[half * NBUF + buf], bph);
-                        if (!ok) break;
                         tc_fence_after();
                         tbase = tmem_base + ((uint32_t)(eg * 32) << 16) + (uint32_t)((half * NBUF + buf) * (BN / NH));
+                    };
+                    if (__builtin_expect(wide, 0)) {
+#pragma unroll 1
+                        for (int j = 0; j < n; ++j) {
+                            ready();
+                            if (!ok) break;
+                            const float x = ld_shared_f32(sc + (eg * 32 + lane) * 16 + 4 * j);
+                            float t0, t1;
+                            const float f0 = split_scale(x, ld_shared_f32(sc + 2048 + 4 * j), t0);
+                            const float f1 = split_scale(x, ld_shared_f32(sc + 2064 + 4 * j), t1);
+#pragma unroll
+                            for (int c = 0; c < 4 * CH; ++c) {
+                                const float f = c / 4 < CPH ? f0 : f1, t = c / 4 < CPH ? t0 : t1;
+                                float p[8];
+                                tmem_ld8f(tbase + acol(c / 4) + c % 4 * 8, p);
+                                tmem_wait_ld();
+                                if (c == 4 * CH - 1) release();
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    fma_f32x2(acc[c / 4][c % 4 * 4 + i], make_float2(p[2 * i] * f, p[2 * i + 1] * f),
+                                              make_float2(t, t));
+                            }
+                        }
+                        used();
+                        continue;
+                    }
+                    used();
+#pragma unroll 1
+                    for (int j = 0; j < n; ++j) {
+                        ready();
+                        if (!ok) break;
                         // A chunk loads while the one before it is added; the accumulator is handed back before
                         // the last additions.
                         float p0[32], p1[32];
@@ -1122,14 +1225,15 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
             // lane = (unit, half of a gated unit, block of K)
             const int first = (tl.n0 + (lane >> 3)) * (glu ? 16 : 32);
             const int nb = glu ? (first >> 7) * 2 + ((lane >> 2) & 1) : first >> 7;
-            const float *ws = a.ws + tl.e * a.ws_group + (int64_t)min(nb, a.ws_blocks - 1) * a.ld_ws + (lane & 3);
+            const float *ws = a.ws + tl.e * a.ws_group + (int64_t)min(nb, a.ws_blocks - 1) * a.ld_ws;
             for (int kb = 0; kb < a.num_k; kb += kScaleQuad) {
                 ok = wait(&sempty[slot], ph ^ 1u, ERR_SITE_BLOCKS_PRODUCER);
                 if (!ok) break;
                 uint8_t *d = smem + C::SCALE_OFF + slot * C::SLOT_BYTES;
-                const int n = min(kScaleQuad, a.num_k - kb);
-                for (int j = 0; j < n; ++j) cp_async_4(d + (j * C::ROWS + lane) * 4, xs + kb + j);
-                if ((lane & 3) < n) cp_async_4(d + kScaleQuad * C::ROWS * 4 + lane * 4, ws + kb);
+                const int n = min(kScaleQuad, a.num_k - kb);  // past the last block its scales again
+#pragma unroll
+                for (int j = 0; j < kScaleQuad; ++j) cp_async_4(d + (j * C::ROWS + lane) * 4, xs + kb + min(j, n - 1));
+                cp_async_4(d + kScaleQuad * C::ROWS * 4 + lane * 4, ws + kb + min(lane & 3, n - 1));
                 cp_async_arrive(&sfull[slot]);
                 if (++slot == SLOTS) {
                     slot = 0;
@@ -1171,7 +1275,7 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
                     const uint32_t sc = scales + slot * C::SLOT_BYTES;
                     const int n = min(kScaleQuad, a.num_k - kb);
                     // Four blocks of K a hand-over: one at a time, its waits and loads took 420 cycles each.
-                    auto add = [&](auto count) {
+                    auto add = [&](auto count, auto is_wide) {
                         constexpr int R = decltype(count)::value;
                         float p[kScaleQuad][R], w[4];
 #pragma unroll
@@ -1192,16 +1296,41 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
                                 float x[4];
                                 ld_shared_v4(sc + (j * C::ROWS + 4 * q) * 4, x);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) v[4 * q + i] = fmaf(p[j][4 * q + i], w[j] * x[i], v[4 * q + i]);
+                                for (int i = 0; i < 4; ++i) {
+                                    float &t = v[4 * q + i];
+                                    if constexpr (decltype(is_wide)::value)
+                                        t += (float)((double)p[j][4 * q + i] * ((double)w[j] * (double)x[i]));
+                                    else
+                                        t = fmaf(p[j][4 * q + i], w[j] * x[i], t);
+                                }
                             }
                         }
                     };
+                    // Whether the scale of one of them is wide: lane (j, q) looks at rows 4 q .. 4 q + 3 in block j.
+                    auto any_wide = [&]() {
+                        float x[4];
+                        ld_shared_v4(sc + lane * 16, x);
+                        const uint32_t at = sc + kScaleQuad * C::ROWS * 4 + unit * 32 + (lane >> 3) * 4;
+                        const float w0 = ld_shared_f32(at), w1 = ld_shared_f32(at + 16);
+                        float least = fabsf(x[0]), most = least;
+#pragma unroll
+                        for (int i = 1; i < 4; ++i) least = fminf(least, fabsf(x[i])), most = fmaxf(most, fabsf(x[i]));
+                        least *= fminf(fabsf(w0), fabsf(w1));
+                        most *= fmaxf(fabsf(w0), fabsf(w1));
+                        if (__builtin_expect(__all_sync(0xffffffffu, ordinary_scales(least, most)), 1)) return false;
+                        bool wide = false;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) wide = wide || wide_scale(x[i], w0) || wide_scale(x[i], w1);
+                        return __any_sync(0xffffffffu, wide) != 0;
+                    };
                     if (!mine)
                         release();
+                    else if (__builtin_expect(any_wide(), 0))  // in 64 bits, for few such calls
+                        add(std::integral_constant<int, 32>{}, std::true_type{});
                     else if (tl.rows <= 8)
-                        add(std::integral_constant<int, 8>{});
+                        add(std::integral_constant<int, 8>{}, std::false_type{});
                     else
-                        add(std::integral_constant<int, 32>{});
+                        add(std::integral_constant<int, 32>{}, std::false_type{});
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sempty[slot]);
                     if (++slot == SLOTS) {
