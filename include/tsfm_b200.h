@@ -311,7 +311,7 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
  *   [ceil(rows / block_rows), ceil(cols / 128)] with row stride ld_scale. x[r, c] ~ q[r, c] * scale:
  *   the scale is the smallest power of two with max|x| / scale <= 448 (at least 2^-126), q =
  *   x / scale rounded to nearest even. A block that holds an infinity or a NaN gets scale and codes
- *   NaN. rows may be 0.
+ *   NaN. rows may be 0 (x, q and scale may then be null).
  *
  * tsfm_kernel_linear_e4m3: y[M, N] (+)= act(x W^T + bias) of E4M3 operands x [M, K] and W [N, K]
  *   (row strides ldx, ldw in bytes, both and the bases 16-byte aligned; K itself may be odd) with
@@ -322,7 +322,7 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
  *   accumulate (F32 only) adds to y, and the activation then applies to the sum. act: 0 none, 1 relu
  *   (a NaN becomes 0, as in tsfm_kernel_linear), 3 gated pairs as there (N % 256 == 0, 16-bit y of
  *   N / 2 columns, no bias).
- *   bias [N] or null. M may be 0. y overlaps no input.
+ *   bias [N] or null. M may be 0 (x, x_scale and y may then be null). y overlaps no input.
  *
  * tsfm_kernel_linear_grouped: y[r] (+)= act(x[r] W[e]^T + bias[e]) for the rows offsets[e] <= r <
  *   offsets[e + 1] of group e, 0 <= e < groups (at most 1024). x [M, K], W [groups, N, K] (row stride

@@ -81,3 +81,16 @@ def test_dtypes_groups_and_empty_batches():
     assert grouped(groups=1025) == "UNSUPPORTED" and grouped_e4m3(groups=1025) == "UNSUPPORTED"
     assert e4m3(M=0) == "OK" and grouped(M=0) == "OK" and grouped_e4m3(M=0) == "OK"
     assert "1024 groups" in (grouped(groups=1025), tb.last_error())[1]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_empty_batches_may_have_null_addresses(dtype):
+    # a tensor without rows has no storage: its x, y, codes and scales are null; weights and offsets are not
+    for block_rows in (1, 128):
+        assert quantize(rows=0, x_dtype=dtype, block_rows=block_rows, x=None, q=None, scale=None) == "OK"
+    assert e4m3(M=0, x=None, xs=None, y=None, y_dtype=dtype) == "OK"
+    assert grouped(M=0, x=None, y=None, y_dtype=dtype) == "OK"
+    assert grouped_e4m3(M=0, x=None, xs=None, y=None, y_dtype=dtype) == "OK"
+    assert e4m3(M=0, w=None) == grouped(M=0, w=None) == grouped(M=0, offsets=None) == "INVALID_ARGUMENT"
+    assert e4m3(M=0, ws=None) == grouped_e4m3(M=0, offsets=None) == "INVALID_ARGUMENT"
+    assert e4m3(M=0, x=None, y=None, act=2) == quantize(rows=0, x=None, cols=0) == "INVALID_ARGUMENT"

@@ -720,7 +720,7 @@ static Status linear_blocks_entry(LinearBlocksCall &c, int64_t groups, int32_t y
     const int64_t ycols = act == ACT_GLU ? c.N / 2 : c.N, kb = (c.K + 127) / 128;
     if (c.ldx < c.K || c.ldw < c.K || c.ldy < ycols || (groups > 1 && c.w_group < (c.N - 1) * c.ldw + c.K))
         return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: a stride is shorter than its rows");
-    if (f8 && (!c.xs || !c.ws || c.ld_xs < kb || c.ld_ws < kb ||
+    if (f8 && ((c.M > 0 && !c.xs) || !c.ws || c.ld_xs < kb || c.ld_ws < kb ||
                (groups > 1 && c.ws_group < ((c.N + 127) / 128 - 1) * c.ld_ws + kb)))
         return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: bad scales");
     const int esz = f8 ? 1 : 2, ysz = y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
@@ -741,7 +741,8 @@ static Status linear_blocks_entry(LinearBlocksCall &c, int64_t groups, int32_t y
 int32_t tsfm_kernel_quantize_e4m3(const void *x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t ldx,
                                   int32_t block_rows, void *q, int64_t ldq, float *scale, int64_t ld_scale, void *stream) {
     return guarded([&]() -> Status {
-        if (!x || !q || !scale) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        // An empty tensor's address may be null.
+        if (rows > 0 && (!x || !q || !scale)) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
         if (x_dtype != TSFM_DTYPE_F32 && x_dtype != TSFM_DTYPE_F16 && x_dtype != TSFM_DTYPE_BF16)
             return Status::fail(TSFM_ERR_UNSUPPORTED_DTYPE, "quantize: x must be F32, F16 or BF16");
         if (rows < 0 || cols <= 0 || rows > INT32_MAX || cols > INT32_MAX || ldx < cols || ldq < cols ||
@@ -769,7 +770,7 @@ int32_t tsfm_kernel_linear_e4m3(const void *x, const float *x_scale, int64_t ld_
                                 int32_t act, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldy,
                                 void *stream) {
     return guarded([&]() -> Status {
-        if (!x || !w || !y) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        if (!w || (M > 0 && (!x || !y))) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
         LinearBlocksCall c;
         c.x = x;
         c.w = w;
@@ -795,7 +796,7 @@ int32_t tsfm_kernel_linear_grouped(const void *x, int32_t x_dtype, const void *w
                                    int64_t groups, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw,
                                    int64_t w_group, int64_t ldy, void *stream) {
     return guarded([&]() -> Status {
-        if (!x || !w || !y || !offsets) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        if (!w || !offsets || (M > 0 && (!x || !y))) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
         if (x_dtype != w_dtype || (x_dtype != TSFM_DTYPE_BF16 && x_dtype != TSFM_DTYPE_F16))
             return Status::fail(TSFM_ERR_UNSUPPORTED_DTYPE, "linear: x and w must both be BF16 or F16");
         LinearBlocksCall c;
@@ -822,7 +823,7 @@ int32_t tsfm_kernel_linear_grouped_e4m3(const void *x, const float *x_scale, int
                                         int64_t groups, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw,
                                         int64_t w_group, int64_t ldy, void *stream) {
     return guarded([&]() -> Status {
-        if (!x || !w || !y || !offsets) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
+        if (!w || !offsets || (M > 0 && (!x || !y))) return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "null pointer");
         LinearBlocksCall c;
         c.x = x;
         c.w = w;
