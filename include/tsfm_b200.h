@@ -353,18 +353,26 @@ int32_t tsfm_kernel_linear_grouped_e4m3(const void *x, const float *x_scale, int
                                         int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t w_group,
                                         int64_t ldy, void *stream);
 
-/* tsfm_test_bounded_wait: the failure-detection check of the device waits. Every wait of the
- * warp-specialised kernels (TMA and tensor-core barriers) gives up after 2 s, records its site in
- * the device error word and lets the kernel return, and the host reports
- * TSFM_ERR_DEVICE_TIMEOUT; this entry runs that same bounded wait on a barrier that nothing
- * arrives on, with a limit of limit_ns (1 us .. 2 s), and returns what the host then reports
- * (TSFM_ERR_DEVICE_TIMEOUT). The context stays usable. No counterpart in the reference (its GPU
- * seam has no device waits).
+/* tsfm_kernel_status: whether a kernel of the entry points in this section gave up. Every wait of the
+ * warp-specialised kernels (TMA and tensor-core barriers) gives up after 2 s, records its site in the
+ * device's error word and lets the kernel return, with outputs that are not all written; the call that
+ * launched it has returned by then, and nothing else tells its caller. This entry waits for `stream`,
+ * returns TSFM_ERR_DEVICE_TIMEOUT if the word was set (by any stream of the current device since the last
+ * report) and clears it. Not on a stream that is being captured. The forecasts and the GEMM seam look
+ * at words of their own and report by themselves. */
+int32_t tsfm_kernel_status(void *stream);
+
+/* tsfm_test_bounded_wait: the failure-detection check of the device waits: that same bounded wait on a
+ * barrier that nothing arrives on, with a limit of limit_ns (1 us .. 2 s), and what the host then
+ * reports (TSFM_ERR_DEVICE_TIMEOUT); tsfm_test_bounded_wait_enqueue: the wait alone, as a kernel of the
+ * entry points makes it, for tsfm_kernel_status to report. The context stays usable. No
+ * counterpart in the reference (its GPU seam has no device waits).
  * Host-side failure injection: with the environment variable TSFM_FAIL_REPLICA=<i>, the forecast
  * worker of replica i of a multi-device model fails before touching its device while the other
  * workers run and are joined (the forecast returns TSFM_ERR_INVALID_ARGUMENT); unset in normal
  * use. */
 int32_t tsfm_test_bounded_wait(int64_t limit_ns, void *stream);
+int32_t tsfm_test_bounded_wait_enqueue(int64_t limit_ns, void *stream);
 
 /* The corrected product's pieces on device pointers, for benches and tests that time the product
  * alone: tsfm_kernel_split_f16c writes x16 = f16(x) [rows, cols] and its FP8 companion x8

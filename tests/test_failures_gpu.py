@@ -63,3 +63,31 @@ def test_one_replica_worker_fails_others_join(family, monkeypatch):
     assert e.value.name == "INVALID_ARGUMENT" and "injected failure" in str(e.value)
     monkeypatch.delenv("TSFM_FAIL_REPLICA")
     assert np.array_equal(run(), want)
+
+
+def test_kernel_status_reports_a_wait_that_gave_up_once():
+    # a kernel-level call returns after enqueueing: what became of its waits is what tsfm_kernel_status says
+    side = torch.cuda.Stream()
+    cur = torch.cuda.current_stream().cuda_stream
+    assert tb.lib.tsfm_kernel_status(cur) == 0
+    assert tb.lib.tsfm_test_bounded_wait_enqueue(2_000_000, side.cuda_stream) == 0
+    # the synchronous check has a word of its own and takes no other call's report away
+    assert tb.STATUS_NAMES[tb.lib.tsfm_test_bounded_wait(1_000_000, side.cuda_stream)] == "DEVICE_TIMEOUT"
+    st = tb.lib.tsfm_kernel_status(side.cuda_stream)
+    assert tb.STATUS_NAMES[st] == "DEVICE_TIMEOUT" and "gave up (site 0x0301)" in tb.last_error()
+    assert tb.lib.tsfm_kernel_status(side.cuda_stream) == 0
+    # products afterwards run and report nothing; a captured wait reports at its replay
+    x = torch.ones(64, 64, device="cuda", dtype=torch.bfloat16)
+    y = torch.zeros(64, 64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream().cuda_stream
+        assert tb.STATUS_NAMES[tb.lib.tsfm_kernel_status(s)] == "INVALID_ARGUMENT"
+        tb.check(tb.lib.tsfm_kernel_linear(x.data_ptr(), 2, x.data_ptr(), 2, None, y.data_ptr(), 1, 0, 64, 64, 64, 64, 64, 64, s))
+        tb.check(tb.lib.tsfm_test_bounded_wait_enqueue(1_000_000, s))
+    assert tb.lib.tsfm_kernel_status(cur) == 0
+    graph.replay()
+    assert tb.STATUS_NAMES[tb.lib.tsfm_kernel_status(cur)] == "DEVICE_TIMEOUT"
+    assert tb.lib.tsfm_kernel_status(cur) == 0 and (y == 64).all()
+    assert tb.lib.tsfm_test_bounded_wait_enqueue(500, cur) != 0  # limits outside [1 us, 2 s] are refused

@@ -3,6 +3,7 @@
 import pytest
 
 import tsfm_b200 as tb
+from helpers import has_gpu
 
 F32, F16, BF16 = 0, 1, 2
 P = 1 << 20  # an aligned address that no refused call reads
@@ -94,3 +95,12 @@ def test_empty_batches_may_have_null_addresses(dtype):
     assert e4m3(M=0, w=None) == grouped(M=0, w=None) == grouped(M=0, offsets=None) == "INVALID_ARGUMENT"
     assert e4m3(M=0, ws=None) == grouped_e4m3(M=0, offsets=None) == "INVALID_ARGUMENT"
     assert e4m3(M=0, x=None, y=None, act=2) == quantize(rows=0, x=None, cols=0) == "INVALID_ARGUMENT"
+
+
+def test_groups_are_counted_before_anything_else():
+    assert grouped(groups=1025, M=0) == grouped_e4m3(groups=1025, M=0) == "UNSUPPORTED"
+
+
+def test_kernel_status_needs_a_device():
+    # without a device the error word that every product records in cannot be had, and that is an error
+    assert name(tb.lib.tsfm_kernel_status(None)) == ("OK" if has_gpu() else "NO_DEVICE")

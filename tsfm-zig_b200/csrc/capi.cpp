@@ -58,28 +58,58 @@ Status device_count(int *n) {
     return Status::ok();
 }
 
-// Device error words for the kernel-level entry points (one per device, allocated once).
-int *kernel_err_word() {
+// While it lives, this thread's calls are none that a stream capture (its own or another thread's) forbids.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const cudaError_t err = cudaThreadExchangeStreamCaptureMode(&mode);
+    ~RelaxedCapture() {
+        if (err == cudaSuccess) cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+};
+
+// The current device's error words for the kernel-level entry points (allocated once, never freed): [0] for
+// the kernels, read and cleared by tsfm_kernel_status; [1] for tsfm_test_bounded_wait.
+Status kernel_err_word(int **out) {
     static std::mutex mu;
     static int *words[64] = {nullptr};
     int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return nullptr;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver)
+        return Status::fail(TSFM_ERR_NO_DEVICE, std::string("no CUDA device: ") + cudaGetErrorString(e));
+    TSFM_CUDA(e, "error word: device");
+    if (dev < 0 || dev >= 64) return Status::fail(TSFM_ERR_NO_DEVICE, "device ordinal out of range");
     std::lock_guard<std::mutex> lk(mu);
     if (!words[dev]) {
-        // The first call on a device may come from a thread that captures a graph: the allocation runs
-        // in the relaxed capture mode, and the clearing on a stream of its own.
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        // The first call on a device may come from a thread that captures a graph: the clearing runs on a
+        // stream of its own.
+        RelaxedCapture relaxed;
+        TSFM_CUDA(relaxed.err, "error word: capture mode");
         void *p = nullptr;
+        TSFM_CUDA(cudaMalloc(&p, 16), "error word: allocation");
         cudaStream_t s = nullptr;
-        if (cudaMalloc(&p, 16) == cudaSuccess && cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess &&
-            cudaMemsetAsync(p, 0, 16, s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess)
-            words[dev] = static_cast<int *>(p);
+        cudaError_t c = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+        if (c == cudaSuccess) c = cudaMemsetAsync(p, 0, 16, s);
+        if (c == cudaSuccess) c = cudaStreamSynchronize(s);
         if (s) cudaStreamDestroy(s);
-        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (c != cudaSuccess) {
+            cudaFree(p);
+            return Status::cuda(c, "error word: clear");
+        }
+        words[dev] = static_cast<int *>(p);
     }
-    return words[dev];
+    *out = words[dev];
+    return Status::ok();
+}
+
+// What word `err` holds once `st` has caught up; it is cleared.
+Status take_device_error(int *err, cudaStream_t st, const char *what) {
+    int code = 0;
+    TSFM_CUDA(cudaMemcpyAsync(&code, err, sizeof(int), cudaMemcpyDeviceToHost, st), what);
+    TSFM_CUDA(cudaStreamSynchronize(st), what);
+    if (!code) return Status::ok();
+    TSFM_CUDA(cudaMemsetAsync(err, 0, sizeof(int), st), what);
+    TSFM_CUDA(cudaStreamSynchronize(st), what);
+    return Status::fail(TSFM_ERR_DEVICE_TIMEOUT, strf("a kernel's bounded wait gave up (site 0x%04x)", code));
 }
 
 bool is_pinned(const void *p) {
@@ -596,7 +626,7 @@ int32_t tsfm_kernel_linear(const void *x, int32_t x_dtype, const void *w, int32_
         c.out_mode = out_mode == 0 ? out_mode_for(elem) : out_mode == 1 ? OUT_F32 : OUT_F32_ACC;
         c.bias = bias;
         c.act = act;
-        c.err = kernel_err_word();
+        TSFM_TRY(kernel_err_word(&c.err));
         return launch_linear(c, static_cast<cudaStream_t>(stream));
     });
 }
@@ -633,7 +663,7 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
             c.out_mode = out_mode == 0 ? OUT_F16 : out_mode == 1 ? OUT_F32 : OUT_F32_ACC;
             c.bias = bias;
             c.act = act;
-            c.err = kernel_err_word();
+            res = kernel_err_word(&c.err);
             c.x8 = x8;
             c.ldx8 = 2 * K;
             c.w8 = w8;
@@ -642,7 +672,7 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
             c.x8_cols = terms == 1 ? K : 2 * K;
             c.y8 = y8;
             c.ldy8 = 2 * N;
-            res = launch_linear(c, st);
+            if (res) res = launch_linear(c, st);
         }
         cudaFreeAsync(buf, st);
         return res;
@@ -689,7 +719,7 @@ int32_t tsfm_kernel_linear_f16c(const void *x16, const void *x8, const void *w16
         c.out_mode = out_mode == 0 ? OUT_F16 : out_mode == 1 ? OUT_F32 : OUT_F32_ACC;
         c.bias = bias;
         c.act = act;
-        c.err = kernel_err_word();
+        TSFM_TRY(kernel_err_word(&c.err));
         c.x8 = x8;
         c.ldx8 = 2 * K;
         c.w8 = w8;
@@ -729,12 +759,13 @@ static Status linear_blocks_entry(LinearBlocksCall &c, int64_t groups, int32_t y
         return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: operand base and strides must be 16-byte aligned");
     if (off(c.y, ysz) || off(c.bias, 4) || off(c.xs, 4) || off(c.ws, 4) || off(c.offsets, 4))
         return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "linear: misaligned pointer");
+    if (groups > kMaxGroups) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: more than 1024 groups");
     c.groups = groups;
     c.y_dtype = y_dtype;
     c.accumulate = accumulate != 0;
     c.act = act;
     if (c.M == 0) return Status::ok();
-    c.err = kernel_err_word();
+    TSFM_TRY(kernel_err_word(&c.err));
     return launch_linear_blocks(c, stream);
 }
 
@@ -851,18 +882,38 @@ int32_t tsfm_test_bounded_wait(int64_t limit_ns, void *stream) {
     return guarded([&]() -> Status {
         if (limit_ns < 1000 || limit_ns > (int64_t)kWaitTimeoutNs)
             return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "bounded wait: limit outside [1 us, 2 s]");
-        int *err = kernel_err_word();
-        if (!err) return Status::fail(TSFM_ERR_CUDA, "bounded wait: no error word");
+        int *err = nullptr;
+        TSFM_TRY(kernel_err_word(&err));
+        ++err;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        int code = 0;
         TSFM_CUDA(cudaMemsetAsync(err, 0, sizeof(int), st), "bounded wait: clear error word");
         TSFM_TRY(launch_bounded_wait(err, (unsigned long long)limit_ns, st));
-        TSFM_CUDA(cudaMemcpyAsync(&code, err, sizeof(int), cudaMemcpyDeviceToHost, st), "bounded wait: error word");
-        TSFM_CUDA(cudaStreamSynchronize(st), "bounded wait");
-        TSFM_CUDA(cudaMemsetAsync(err, 0, sizeof(int), st), "bounded wait: clear error word");
-        TSFM_CUDA(cudaStreamSynchronize(st), "bounded wait");
-        if (code) return Status::fail(TSFM_ERR_DEVICE_TIMEOUT, strf("a kernel's bounded wait gave up (site 0x%04x)", code));
-        return Status::ok();
+        return take_device_error(err, st, "bounded wait");
+    });
+}
+
+int32_t tsfm_test_bounded_wait_enqueue(int64_t limit_ns, void *stream) {
+    return guarded([&]() -> Status {
+        if (limit_ns < 1000 || limit_ns > (int64_t)kWaitTimeoutNs)
+            return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "bounded wait: limit outside [1 us, 2 s]");
+        int *err = nullptr;
+        TSFM_TRY(kernel_err_word(&err));
+        return launch_bounded_wait(err, (unsigned long long)limit_ns, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t tsfm_kernel_status(void *stream) {
+    return guarded([&]() -> Status {
+        int *err = nullptr;
+        TSFM_TRY(kernel_err_word(&err));
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        TSFM_CUDA(cudaStreamIsCapturing(st, &capture), "kernel status: stream");
+        if (capture != cudaStreamCaptureStatusNone)
+            return Status::fail(TSFM_ERR_INVALID_ARGUMENT, "kernel status: the stream is being captured");
+        RelaxedCapture relaxed;
+        TSFM_CUDA(relaxed.err, "kernel status: capture mode");
+        return take_device_error(err, st, "kernel status");
     });
 }
 
@@ -995,7 +1046,7 @@ int32_t tsfm_kernel_attention_ex(const void *q, const void *k, const void *v, in
         c.ne = mask_mode == 0 ? n : ne;
         c.l = mask_mode == 0 ? n : l;
         c.force_path = force_path;
-        c.err = kernel_err_word();
+        TSFM_TRY(kernel_err_word(&c.err));
         if ((force_path == 1 || force_path == 3) && !attention_tc_supported(c))
             return Status::fail(TSFM_ERR_UNSUPPORTED, "attention: the tcgen05 path does not take this call");
         return launch_attention(c, static_cast<cudaStream_t>(stream));
@@ -1028,7 +1079,7 @@ int32_t tsfm_kernel_attention(const void *q, const void *k, const void *v, int64
         c.dtype = dtype == TSFM_DTYPE_F16 ? E_F16 : E_BF16;
         c.ne = n;
         c.l = n;
-        c.err = kernel_err_word();
+        TSFM_TRY(kernel_err_word(&c.err));
         return launch_attention(c, static_cast<cudaStream_t>(stream));
     });
 }

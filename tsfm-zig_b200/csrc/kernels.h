@@ -305,6 +305,8 @@ struct QuantizeCall {
 };
 Status launch_quantize_e4m3(const QuantizeCall &c, cudaStream_t stream);
 
+constexpr int kMaxGroups = 1024;  // of a grouped product: two words of shared memory each
+
 // Products over block-scaled E4M3 operands, and products grouped by expert (linear_blocks.cu):
 // y[r] (+)= act(x[r] W[e]^T + bias[e]) for the rows r of group e.
 struct LinearBlocksCall {

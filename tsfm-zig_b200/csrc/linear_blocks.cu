@@ -63,8 +63,6 @@ namespace tsfm {
 
 namespace {
 
-constexpr int kMaxGroups = 1024;  // two words of shared memory each
-
 // Blocks of K whose scales share a slot of the ring, and the slots.
 constexpr int kScaleQuad = 4, kScaleSlots = 4;
 constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2 + 1) * 4;  // [row][block of K], [half tile][block of K], wide
@@ -1569,7 +1567,6 @@ Status launch_kind(const LinearBlocksCall &c, cudaStream_t stream) {
 }  // namespace
 
 Status launch_linear_blocks(const LinearBlocksCall &c, cudaStream_t stream) {
-    if (c.groups > kMaxGroups) return Status::fail(TSFM_ERR_UNSUPPORTED, "linear: more than 1024 groups");
     switch (c.dtype) {
         case E_U8: return launch_kind<E_U8>(c, stream);
         case E_F16: return launch_kind<E_F16>(c, stream);
