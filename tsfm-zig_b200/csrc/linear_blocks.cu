@@ -1419,14 +1419,17 @@ BlkArgs blk_args(const LinearBlocksCall &c, int n_tiles, int bk) {
     return a;
 }
 
-// x by boxes of `rows` rows and W [groups, N, K] by boxes of w_rows rows; for gated pairs W is [groups,
-// N / 256, 2, 128, K] and a box holds w_rows rows of each of w_halves of them.
-Status operand_maps(const LinearBlocksCall &c, int kind, uint32_t bk, uint32_t rows, uint32_t w_rows, uint32_t w_halves,
-                    CUtensorMap *tx, CUtensorMap *tw) {
-    const bool glu = c.act == ACT_GLU;
+// x by boxes of `rows` rows.
+Status x_map(const LinearBlocksCall &c, int kind, uint32_t bk, uint32_t rows, CUtensorMap *tx) {
     const int64_t dx[2] = {c.K, c.M}, sx[2] = {1, c.ldx};
     const uint32_t bx[2] = {bk, rows};
-    TSFM_TRY(make_tmap_nd(tx, c.x, kind, 2, dx, sx, bx));
+    return make_tmap_nd(tx, c.x, kind, 2, dx, sx, bx);
+}
+
+// W [groups, N, K] by boxes of w_rows rows; for gated pairs W is [groups, N / 256, 2, 128, K] and a box holds
+// w_rows rows of each of w_halves of them.
+Status w_map(const LinearBlocksCall &c, int kind, uint32_t bk, uint32_t w_rows, uint32_t w_halves, CUtensorMap *tw) {
+    const bool glu = c.act == ACT_GLU;
     const int64_t wg = c.groups > 1 ? c.w_group : c.N * c.ldw;
     const int64_t dw[5] = {c.K, glu ? 128 : c.N, glu ? 2 : 1, glu ? c.N / 256 : 1, c.groups};
     const int64_t sw[5] = {1, c.ldw, glu ? 128 * c.ldw : c.N * c.ldw, glu ? 256 * c.ldw : c.N * c.ldw, wg};
@@ -1445,9 +1448,15 @@ Status launch_few(const LinearBlocksCall &c, cudaStream_t stream) {
     constexpr int BK = C::F8 ? 128 : 64;
     alignas(64) CUtensorMap tx, tw, tw4;
     const bool glu = c.act == ACT_GLU;
-    TSFM_TRY(operand_maps(c, KIND, BK, C::ROWS, glu ? 16 : 32, glu ? 2 : 1, &tx, &tw));
-    tw4 = tw;
-    if (!glu) TSFM_TRY(operand_maps(c, KIND, BK, C::ROWS, 128, 1, &tx, &tw4));
+    TSFM_TRY(x_map(c, KIND, BK, C::ROWS, &tx));
+    // W by units (gated pairs, and the tiles of fewer than four) and by whole tiles: those of the two that
+    // this N has.
+    const int64_t units = (c.N + 31) / 32;
+    const bool by_unit = glu || units % 4 != 0, by_tile = !glu && units >= 4;
+    if (by_unit) TSFM_TRY(w_map(c, KIND, BK, glu ? 16 : 32, glu ? 2 : 1, &tw));
+    if (by_tile) TSFM_TRY(w_map(c, KIND, BK, 128, 1, &tw4));
+    if (!by_unit) tw = tw4;
+    if (!by_tile) tw4 = tw;
     const BlkArgs a = blk_args(c, (int)((c.N + 127) / 128), BK);
     const int smem = C::smem(c.groups);
     TSFM_TRY(ensure_smem_attr(reinterpret_cast<const void *>(&linear_few_rows_kernel<KIND>), smem));
@@ -1466,7 +1475,8 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
     constexpr int BK = C::F8 ? 128 : 64;
     alignas(64) CUtensorMap ta, tb, ty;
     const bool glu = c.act == ACT_GLU;
-    TSFM_TRY(operand_maps(c, KIND, BK, C::A_BOX, PAIR || glu ? BN / 2 : BN, !PAIR && glu ? 2 : 1, &ta, &tb));
+    TSFM_TRY(x_map(c, KIND, BK, C::A_BOX, &ta));
+    TSFM_TRY(w_map(c, KIND, BK, PAIR || glu ? BN / 2 : BN, !PAIR && glu ? 2 : 1, &tb));
     BlkArgs a = blk_args(c, (int)((c.N + BN - 1) / BN), BK);
     const int ysz = c.y_dtype == TSFM_DTYPE_F32 ? 4 : 2;
     a.vec = reinterpret_cast<uintptr_t>(c.y) % (4 * ysz) == 0 && c.ldy % 4 == 0;
