@@ -1,12 +1,13 @@
 """The block-scaled and grouped products where their inputs leave the ordinary range, on every tile form
 that the sizes choose: gates far below zero, scales whose product leaves FP32, non-finite values and
 partial boxes on pairs of SMs, streams that join, a quantiser past 2^31 elements."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import tsfm_b200 as tb  # noqa: E402
-from test_linear_blocks_gpu import E4M3, Case, gen  # noqa: E402
+from test_linear_blocks_gpu import E4M3, Case, gen, ptr, quantize  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +143,128 @@ def test_partial_boxes_leave_the_padding(M, N, K):
         c.check(dtype, pad=-N % 8 + 8, shift=8)
     g = Case(M, N, K, "e4m3", counts=[M // 2, 0, 3, M - M // 2 - 10], first=4, bias=True, seed=25)
     g.check(torch.bfloat16, pad=-N % 8 + 24)
+
+
+@pytest.mark.parametrize("act", [0, 1, 3])
+@pytest.mark.parametrize("kind", ["e4m3", torch.bfloat16], ids=str)
+def test_nonfinite_values_on_pairs_of_sms(kind, act):
+    # rows and columns of NaN and infinities on 256 x 256 tiles: through the boxes (16-bit y), and past them
+    counts = [4000, 0, 3500, 1500]
+    M, N, K = sum(counts), 2048, 1024
+    c = Case(M, N, K, kind, counts=counts, seed=23)
+    if act == 3:
+        k = 0.5 / float(c.ref.std())
+        (c.xs if kind == "e4m3" else c.x).mul_(k)
+    cols = N // 2 if act == 3 else N
+    dtypes = (torch.bfloat16,) if act == 3 else (torch.bfloat16, torch.float32)
+    clean = {}
+    for dtype in dtypes:
+        for pad in (0, 4):
+            clean[dtype, pad] = torch.zeros(M, cols + pad, device="cuda", dtype=dtype)
+            tb.check(c.call(clean[dtype, pad], act=act))
+    c.x[45, 7] = float("nan")
+    if kind == "e4m3":
+        c.xs[7777, 1] = float("inf")
+    else:
+        c.x[7777, 200] = float("inf")
+    c.w[2, 20, 3] = float("nan")        # gated: g of column 20; else column 20
+    c.w[2, 256 + 128 + 71, 9] = float("nan")  # gated: u of column 128 + 71
+    hit = torch.zeros(cols, dtype=torch.bool, device="cuda")
+    hit[[20, 199] if act == 3 else [20, 455]] = True
+    keep = torch.ones(M, cols, dtype=torch.bool, device="cuda")
+    keep[45] = keep[7777] = False
+    keep[4000:7500, hit] = False
+    for (dtype, pad), want in clean.items():
+        y = torch.zeros_like(want)
+        tb.check(c.call(y, act=act))
+        torch.cuda.synchronize()
+        assert torch.equal(y[:, :cols][keep], want[:, :cols][keep])
+        if act == 1:  # a NaN becomes 0
+            assert (y[45] == 0).all() and (y[4000:7500, :cols][:, hit] == 0).all()
+            assert not (torch.isfinite(y[7777, :cols]) & (y[7777, :cols] != 0)).any()
+        else:
+            assert torch.isnan(y[45, :cols]).all() and torch.isnan(y[4000:7500, :cols][:, hit]).all()
+            assert not (torch.isfinite(y[7777, :cols]) & (y[7777, :cols] != 0)).any()
+
+
+def test_streams_that_join():
+    # A product whose operands come from kernels of two streams that meet by an event, eager and captured, and
+    # whose output a third call overwrites at once.
+    M, N, K = 2500, 1024, 768
+    g = gen(26)
+    x = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    w = torch.randn(N, K, generator=g, device="cuda").bfloat16()
+    xq, xs = torch.zeros(M, K, dtype=torch.uint8, device="cuda"), torch.zeros(M, K // 128, device="cuda")
+    wq, ws = torch.zeros(N, K, dtype=torch.uint8, device="cuda"), torch.zeros(N // 128, K // 128, device="cuda")
+    y, copy = torch.zeros(M, N, device="cuda"), torch.zeros(M, N, device="cuda")
+    side = torch.cuda.Stream()
+
+    def steps(pause):
+        main = torch.cuda.current_stream()
+        xq.zero_(), xs.zero_(), wq.zero_(), ws.zero_(), y.zero_()
+        side.wait_stream(main)
+        pause()
+        tb.check(tb.lib.tsfm_kernel_quantize_e4m3(ptr(w), 2, N, K, K, 128, ptr(wq), K, ptr(ws), K // 128, side.cuda_stream))
+        tb.check(tb.lib.tsfm_kernel_quantize_e4m3(ptr(x), 2, M, K, K, 1, ptr(xq), K, ptr(xs), K // 128, main.cuda_stream))
+        main.wait_stream(side)
+        pause()
+        tb.check(tb.lib.tsfm_kernel_linear_e4m3(ptr(xq), ptr(xs), K // 128, ptr(wq), ptr(ws), K // 128, None, ptr(y), 0, 0, 0,
+                                                M, N, K, K, K, N, main.cuda_stream))
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            copy.copy_(y)
+        main.wait_stream(side)
+        pause()
+        tb.check(tb.lib.tsfm_kernel_linear_e4m3(ptr(xq), ptr(xs), K // 128, ptr(wq), ptr(ws), K // 128, None, ptr(y), 0, 1, 0,
+                                                M, N, K, K, K, N, main.cuda_stream))
+
+    steps(torch.cuda.synchronize)
+    torch.cuda.synchronize()
+    want = y.clone(), copy.clone()
+    assert want[1].abs().max() > 0 and torch.equal(want[0], 2 * want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps(lambda: None)
+    for how in (lambda: steps(lambda: None), graph.replay) * 5:
+        y.fill_(-1.0), copy.fill_(-1.0)
+        how()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(copy, want[1])
+
+
+@pytest.mark.parametrize("kind", ["e4m3", torch.bfloat16], ids=str)
+def test_large_grouped_products_repeat_themselves(kind):
+    # 32768 rows over 24 of 32 groups, gated: the same bits from every call, alone and in a row
+    g = gen(27)
+    counts = (torch.rand(32, generator=g, device="cuda") ** 2 * (torch.arange(32, device="cuda") % 4 != 1)).cpu().numpy()
+    counts = np.floor(counts / counts.sum() * 32768).astype(int)
+    counts[0] += 32768 - counts.sum()
+    c = Case(32768, 4096, 1024, kind, counts=counts.tolist(), seed=28)
+    k = 0.5 / float(c.ref.std())
+    (c.xs if kind == "e4m3" else c.x).mul_(k)
+    want = torch.zeros(32768, 2048, device="cuda", dtype=torch.bfloat16)
+    tb.check(c.call(want, act=3))
+    torch.cuda.synchronize()
+    ys = [torch.zeros_like(want) for _ in range(8)]
+    for y in ys:
+        tb.check(c.call(y, act=3))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in ys)
+
+
+def test_quantize_past_32_bits():
+    # more than 2^31 elements: the last rows and scales
+    rows, cols = 1050000, 2056
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    tail = torch.randn(200, cols, generator=gen(29), device="cuda").bfloat16()
+    x[-200:] = tail
+    for block_rows in (1, 128):
+        q, s = quantize(x, block_rows)
+        first = rows - 200 - (rows - 200) % block_rows  # of the last 200 rows' blocks
+        part = x[first:].clone()
+        qw, sw = quantize(part, block_rows)
+        assert torch.equal(q[first:], qw) and torch.equal(s[first // block_rows:], sw)
+        assert qw[-1].any() and (q[:first] == 0).all() and (s[:first // block_rows] == 2.0 ** -126).all()
+        del q, s
+    del x
+    torch.cuda.empty_cache()
