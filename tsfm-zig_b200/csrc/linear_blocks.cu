@@ -1273,7 +1273,7 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
                     const uint32_t sc = scales + slot * C::SLOT_BYTES;
                     const int n = min(kScaleQuad, a.num_k - kb);
                     // Four blocks of K a hand-over: one at a time, its waits and loads took 420 cycles each.
-                    auto add = [&](auto count, auto is_wide) {
+                    auto add = [&](auto count) {
                         constexpr int R = decltype(count)::value;
                         float p[kScaleQuad][R], w[4];
 #pragma unroll
@@ -1294,13 +1294,7 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
                                 float x[4];
                                 ld_shared_v4(sc + (j * C::ROWS + 4 * q) * 4, x);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    float &t = v[4 * q + i];
-                                    if constexpr (decltype(is_wide)::value)
-                                        t += (float)((double)p[j][4 * q + i] * ((double)w[j] * (double)x[i]));
-                                    else
-                                        t = fmaf(p[j][4 * q + i], w[j] * x[i], t);
-                                }
+                                for (int i = 0; i < 4; ++i) v[4 * q + i] = fmaf(p[j][4 * q + i], w[j] * x[i], v[4 * q + i]);
                             }
                         }
                     };
@@ -1321,14 +1315,32 @@ __global__ void __launch_bounds__((FewCfg<KIND>::THREADS), 1)
                         for (int i = 0; i < 4; ++i) wide = wide || wide_scale(x[i], w0) || wide_scale(x[i], w1);
                         return __any_sync(0xffffffffu, wide) != 0;
                     };
+                    // Then, a block at a time, in 64 bits.
+                    auto add_wide = [&]() {
+#pragma unroll 1
+                        for (int j = 0; j < n; ++j) {
+                            float p[32];
+                            tmem_ld32f(tbase() + j * C::ROWS, p);
+                            const double w = ld_shared_f32(sc + kScaleQuad * C::ROWS * 4 + (unit * 2 + (lane >> 4)) * 16 + 4 * j);
+                            tmem_wait_ld();
+                            if (j == n - 1) release();
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                float x[4];
+                                ld_shared_v4(sc + (j * C::ROWS + 4 * q) * 4, x);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[4 * q + i] += (float)((double)p[4 * q + i] * (w * (double)x[i]));
+                            }
+                        }
+                    };
                     if (!mine)
                         release();
-                    else if (__builtin_expect(any_wide(), 0))  // in 64 bits, for few such calls
-                        add(std::integral_constant<int, 32>{}, std::true_type{});
+                    else if (__builtin_expect(any_wide(), 0))
+                        add_wide();
                     else if (tl.rows <= 8)
-                        add(std::integral_constant<int, 8>{}, std::false_type{});
+                        add(std::integral_constant<int, 8>{});
                     else
-                        add(std::integral_constant<int, 32>{}, std::false_type{});
+                        add(std::integral_constant<int, 32>{});
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sempty[slot]);
                     if (++slot == SLOTS) {
