@@ -18,7 +18,7 @@
 //   warp 2      E4M3, 256 columns: issues the TMA stores of the boxes that the epilogue fills.
 //   warp 3      E4M3: the scales of the tile's rows and columns into a ring of shared memory, four
 //               blocks of K at a time, ahead of the tiles that need them, marked where a product of two
-//               of them leaves FP32 (the mark costs the 256-wide tiles 2 %; looked for by the epilogue, 4 %).
+//               of them leaves FP32 (this costs the 256-wide tiles 1.3 to 2 %; looked for by the epilogue, 4 %).
 //   warps 4..   epilogue: a thread owns a row and 128 (below 256 columns: 64) of its columns, which
 //               are whole 32-byte sectors of y (columns past N, other alignments and sums into y pass
 //               through 4 KB of shared memory a warp). E4M3 on 256 columns with a 16-bit y: through
@@ -65,7 +65,10 @@ namespace {
 
 // Blocks of K whose scales share a slot of the ring, and the slots.
 constexpr int kScaleQuad = 4, kScaleSlots = 4;
-constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2 + 1) * 4;  // [row][block of K], [half tile][block of K], wide
+constexpr int kScaleSlotBytes = kScaleQuad * (128 + 2 + 1) * 4;  // [row][block of K], [half tile][block of K], spare
+// In place of W's first scale, which is then in the spare words: a scale of the slot is wide. (A NaN that no
+// arithmetic gives; a caller's own is treated as a mark.)
+constexpr uint32_t kWideMark = 0x7fedcba9u;
 
 // KIND: element type of x and W (E_F16, E_BF16, E_U8 = E4M3).
 template <int KIND, int BN>
@@ -618,7 +621,10 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     wide = __any_sync(0xffffffffu, wide) != 0;
                 }
                 if (lane == 0) {
-                    st_shared_f32(d + 2080, wide ? 1.0f : 0.0f);
+                    if (wide || __float_as_uint(w0[0]) == kWideMark) {
+                        st_shared_f32(d + 2080, w0[0]);
+                        st_shared_f32(d + 2048, __uint_as_float(kWideMark));
+                    }
                     mbar_arrive(&sfull[landing]);
                 }
             };
@@ -715,7 +721,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                     ld_shared_v4(sc + (eg * 32 + lane) * 16, xv);
                     ld_shared_v4(sc + 2048, w0);
                     ld_shared_v4(sc + 2064, w1);
-                    const bool wide = ld_shared_f32(sc + 2080) != 0.0f;
+                    const bool wide = __float_as_uint(w0[0]) == kWideMark;
 #pragma unroll
                     for (int j = 0; j < kScaleQuad; ++j) s0[j] = xv[j] * w0[j], s1[j] = xv[j] * w1[j];
                     const int n = min(kScaleQuad, kbn - kb);
@@ -739,7 +745,7 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
                             if (!ok) break;
                             const float x = ld_shared_f32(sc + (eg * 32 + lane) * 16 + 4 * j);
                             float t0, t1;
-                            const float f0 = split_scale(x, ld_shared_f32(sc + 2048 + 4 * j), t0);
+                            const float f0 = split_scale(x, ld_shared_f32(sc + (j ? 2048 + 4 * j : 2080)), t0);
                             const float f1 = split_scale(x, ld_shared_f32(sc + 2064 + 4 * j), t1);
 #pragma unroll
                             for (int c = 0; c < 4 * CH; ++c) {
