@@ -271,8 +271,10 @@ int32_t tsfm_sgemm_nt_noalloc(int m, int n, int k, float alpha, const float *A, 
                               const float *B, int ldb, float *C, int ldc, void *stream);
 
 /* ---------------------------------------------------------------------------------------------
- * Kernel-level entry points on device pointers (what the family forwards are built from; used by
- * the kernel parity tests). All return after enqueueing on `stream`.
+ * Kernel-level entry points on device pointers: what the family forwards are built from (for the kernel
+ * parity tests), and products for a caller's own layers (block-scaled 8-bit and grouped ones, below),
+ * which no family here uses. All return after enqueueing on `stream`; tsfm_kernel_status reports a
+ * kernel that gave up.
  *
  * tsfm_kernel_linear: y[M, N] (+)= act(x[M, K] · W[N, K]^T + bias) on the tensor cores.
  *   x_dtype/w_dtype: TSFM_DTYPE_BF16 or TSFM_DTYPE_F16 (kind::f16), or TSFM_DTYPE_F32 (read as
@@ -299,8 +301,9 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
                                      void *y8, int32_t out_mode, int32_t act, int64_t M, int64_t N,
                                      int64_t K, int32_t terms, void *stream);
 
-/* 8-bit operands with a scale per block, and products grouped by expert. Device pointers on the
- * current device; all return after enqueueing on `stream`, allocate nothing on it and can be
+/* 8-bit operands with a scale per block, and products grouped by expert. The caller brings codes and
+ * scales (a checkpoint's, or tsfm_kernel_quantize_e4m3's): the models' tensor tables hold no 8-bit
+ * tensors, and no tsfm_compute mode runs these. Device pointers on the current device; all return after enqueueing on `stream`, allocate nothing on it and can be
  * captured. None has a counterpart in the reference (it has one FP32 product per layer). They are
  * launched as programmatic dependents: a kernel may become resident early, but reads and writes data
  * only after all work ahead of it on the stream has completed.
@@ -326,7 +329,8 @@ int32_t tsfm_kernel_linear_corrected(const float *x, const float *w, const float
  *
  * tsfm_kernel_linear_grouped: y[r] (+)= act(x[r] W[e]^T + bias[e]) for the rows offsets[e] <= r <
  *   offsets[e + 1] of group e, 0 <= e < groups (at most 1024). x [M, K], W [groups, N, K] (row stride
- *   ldw, group stride w_group elements) both BF16 or both F16, bases and strides 16-byte aligned;
+ *   ldw, group stride w_group elements) both BF16 or both F16, bases and strides 16-byte aligned, sums in
+ *   the tensor cores' FP32 (as tsfm_kernel_linear's; they cut additions off, about 1e-9 K of the result);
  *   bias [groups, N] or null; y, accumulate and act as above. offsets: groups + 1 int32 in device
  *   memory, nondecreasing, any group may be empty. Rows of y outside [offsets[0], offsets[groups])
  *   are left as they were. Offsets outside [0, M] are clamped to it, and one below an earlier one is

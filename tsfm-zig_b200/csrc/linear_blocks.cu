@@ -6,7 +6,9 @@
 // The inner sums run on the tensor cores (kind::f8f6f4, FP32 accumulators) one 128-wide block of K
 // at a time; the scales differ from block to block, so each block's sums leave tensor memory and
 // are added, scaled, into FP32 registers. 16-bit operands have no scales: their sums stay in tensor
-// memory over the whole of K.
+// memory over the whole of K. The tensor cores cut each of their additions off, so that FP32 outputs of the
+// 16-bit products end nearer zero by about 1e-9 K of their size (K 256 2.0e-7, K 4096 3.9e-6; E4M3, four
+// additions at a time, 8e-8 in all).
 //
 // One CTA per SM walks tiles of 128 rows x BN columns, BN 64 or 128, or a CTA pair tiles of 256 x 256:
 //   warp 0      TMA producer (and warp 2, for alternate stages, below 256 columns): K-major tiles of x
@@ -31,13 +33,15 @@
 //
 // What bounds it (B200, 148 SMs, random operands):
 //   16 bits, 256 x 256  the tensor cores: their pipe is active 82 % of the time at M 16384, N 4096,
-//                       K 1024 in 16 groups, 1530 TFLOP/s at M 32768 in 32 groups (179 us); in a row of
-//                       calls the power limit (the same 262,000 cycles at 1.1 to 1.3 GHz, 200 to 235 us).
-//   E4M3, 256 x 256     handing accumulators over: a block of K takes 850 cycles (K 4096: 278 us for
-//                       M 75776, N 1024, 2282 TFLOP/s) where the tensor cores need 512. With nothing
-//                       added to the sums it takes 705, with one load a pass 693: two accumulators a half
-//                       and 1390 cycles for one's round (MMA, commit, wait, loads, hand-back). At K 768 a
-//                       tile's finish is 1500 of 7200 cycles (1636 TFLOP/s at M 73856, N 2304, 160 us).
+//                       K 1024 in 16 groups; M 32768 in 32 groups takes 179 to 190 us after a pause (1450
+//                       to 1530 TFLOP/s), in a row of calls what the power limit leaves (the same 266,000
+//                       cycles at 1.06 to 1.3 GHz, 200 to 250 us).
+//   E4M3, 256 x 256     handing accumulators over: a block of K takes 880 cycles (K 4096: 297 us for
+//                       M 75776, N 1024, 2140 TFLOP/s) where the tensor cores need 512. When it took
+//                       850, it took 705 with nothing added to the sums, 693 with one load a pass: two
+//                       accumulators a half and 1390 cycles for one's round (MMA, commit, wait, loads,
+//                       hand-back). At K 768 a tile takes 7400 cycles (165 us at M 73856, N 2304, 1580
+//                       TFLOP/s), about 1500 of them its finish.
 //                       128 sums and 64 loaded values a thread leave no room for more warps, 512
 //                       columns of tensor memory none for more accumulators.
 //   few rows            the start and W's bytes; groups of few rows have a kernel of their own below.
@@ -1025,9 +1029,9 @@ __global__ void __launch_bounds__((BlkCfg<KIND, BN>::THREADS), 1)
 // and the 16 of u) by 32 rows of x in turn. Tiles of fewer units, to share the last round evenly, were
 // slower: what an SM receives is its share of the bytes under way, and 200 KB a CTA keep HBM busy through
 // a round that not all SMs have. Loads start before the block has met.
-// Bound by W's bytes and the start. 32 rows over 24 of 32 groups, N 2048, K 1024: E4M3 12.6 us for 51 MB
-// (4.0 TB/s; the first load is issued after 2.2 us, the last has landed after 11 to 12.3), BF16 21.0 us
-// for 101 MB (4.8 TB/s); 128-wide tiles take 19.6 and 23.3.
+// Bound by W's bytes and the start. 32 rows over 24 of 32 groups, N 2048, K 1024: E4M3 12.8 us for 51 MB
+// (4.0 TB/s; the first load is issued after 2.2 us, the last has landed after 11 to 12.3), BF16 21.2 us
+// for 101 MB (4.8 TB/s); 128-wide tiles take 18.9 and 23.1.
 //   warp 0  offsets, TMA producer        warp 1  tensor memory, MMA issue
 //   warp 3  E4M3: scales                 warps 4..7  epilogue, one unit each
 template <int KIND>
@@ -1526,9 +1530,11 @@ Status launch_blk(const LinearBlocksCall &c, int split, cudaStream_t stream) {
 // K and one per tile (units of 100 ns, fitted to M 256-4096, N 768-4096, K 768-4096; the fit need only
 // rank the widths). Groups: each is taken to end in the middle of a tile. Measured, E4M3, us for widths
 // 64 / 128 / 256:
-//   M 512  N 2304 K 768   6.0 /  6.6 / 10.0      M 4096 N 2304 K 768   26.9 / 18.1 / 15.4
-//   M 1024 N 2304 K 768   8.8 /  6.8 / 10.1      M 2048 N 4096 K 1024  26.9 / 20.3 / 17.1
-//   M 2048 N 1024 K 4096 21.9 / 15.0 / 21.5      M 4096 N 1024 K 4096  39.7 / 27.0 / 23.2
+//   M 512  N 2304 K 768   6.3 /  6.9 / 11.0      M 4096 N 2304 K 768   26.9 / 18.4 / 16.5
+//   M 1024 N 2304 K 768   9.1 /  7.1 / 11.2      M 2048 N 4096 K 1024  26.7 / 20.6 / 18.2
+//   M 2048 N 1024 K 4096 22.7 / 15.8 / 23.0      M 4096 N 1024 K 4096  40.2 / 27.5 / 24.3
+// Outside the fit it loses up to 4 % (M 3000 N 2500 K 1024: 24.5 on 128 columns, 25.4 on the 256 taken), and
+// lost 10 to 12 % on three of twenty sizes.
 template <int KIND>
 int tile_width(const LinearBlocksCall &c) {
     struct Cost {
@@ -1558,15 +1564,17 @@ int tile_width(const LinearBlocksCall &c) {
 
 // Whether a call's groups are taken to have few rows. Measured, us on 64- or 128-wide tiles / with the
 // operands exchanged:
-//   E4M3, N 2048 K 1024, 32 groups:  M 32 19.6 / 13.4   M 192 19.6 / 14.9   M 256 (gated) 17.0 / 20.1
-//     all rows in one group:         M 32  8.1 /  8.8   M 128  8.8 /  8.9
-//     4 groups:                      M  4  7.4 /  7.2   M  32  7.5 /  8.1
-//   BF16, the same, 32 groups:       M 32 23.3 / 21.9   M 192 24.1 / 22.6   M 256 (gated) 23.5 / 25.1
-//     4 groups (fewer tiles than SMs, where nothing waits for memory): M 4 8.6 / 9.7
-//   E4M3, one product (N 2304 K 768): M 1 6.4 / 5.8      M 8 6.4 / 6.2       M 16 6.3 / 6.8
-//     K 4096, which a cluster's CTAs share on 64-wide tiles (N 1024): M 1 7.5 / 13.2
-// The host does not know the groups' rows. Rows spread over 192 of 256 groups (M 1536, N 1024, K 512,
-// E4M3) take 50.4 / 30.5, all of them in one group 11.6 / 17.8: the loss is smaller than the gain.
+//   E4M3, N 2048 K 1024, 32 groups:  M 32 18.9 / 12.8   M 192 19.0 / 14.8   M 256 (gated) 16.5 / 18.9
+//     all rows in one group:         M 32  7.5 /  7.8   M 128  8.0 /  8.0
+//     4 groups:                      M  4  7.2 /  6.4   M  32  7.3 /  7.2
+//   BF16, the same, 32 groups:       M 32 23.1 / 21.2   M 192 23.4 / 21.9   M 256 (gated) 22.9 / 24.0
+//     4 groups (fewer tiles than SMs, where nothing waits for memory): M 4 8.2 / 8.9
+//   E4M3, one product (N 2304 K 768): M 1 5.8 / 4.8      M 8 5.8 / 5.1       M 16 5.8 / 5.9
+//     N 2304, longer K:              K 1024 M 1 6.1 / 5.7   M 8 6.1 / 6.0    K 1280 M 1 6.7 / 6.6   M 8 6.6 / 6.9
+//     K 4096, which a cluster's CTAs share on 64-wide tiles (N 1024): M 1 7.0 / 12.0
+// The host does not know the groups' rows. Rows spread over three quarters of the groups, and all of them in one
+// group, E4M3: 256 groups, M 1536, N 1024, K 512 50.0 / 30.8 and 11.3 / 17.1; 1024 groups, M 6144, N 512, K 512
+// 108 / 68 and 29 / 38: the loss is smaller than the gain. BF16: 43.6 / 41.9 and 11.9 / 17.5, 92 / 92 and 29 / 38.
 template <int KIND>
 bool few_rows(const LinearBlocksCall &c) {
     const bool f8 = KIND == E_U8;
@@ -1582,8 +1590,8 @@ Status launch_kind(const LinearBlocksCall &c, cudaStream_t stream) {
     if (bn == 128) return launch_blk<KIND, 128>(c, 1, stream);
     // Few tiles and a long K (one group, 16 blocks of K or more): 2, 4 or 8 CTAs of a cluster share a
     // tile's K, as many as leave all clusters on the card at once (of 8 CTAs, 16 clusters took two
-    // turns). us for 1 / 2 / 4 / 8 CTAs: M 32 N 1024 K 4096 12.6 / 9.7 / 7.7 / 12.9, M 32 N 512 K 8192
-    // 21.0 / 13.9 / 9.7 / 7.9. At K 768 the exchange costs more than it saves (N 2304: 5.9 / 6.3).
+    // turns). us for 1 / 2 / 4 / 8 CTAs: M 32 N 1024 K 4096 12.1 / 8.9 / 7.1 / 12.3, M 32 N 512 K 8192
+    // 20.3 / 12.8 / 8.8 / 7.2. At K 768 the exchange costs more than it saves (N 2304: 5.8 / 5.9).
     int split = 1;
     if (KIND == E_U8 && !c.offsets && c.K >= 2048) {
         const int64_t tiles = ((c.M + 127) / 128) * ((c.N + 63) / 64);
